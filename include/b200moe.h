@@ -302,6 +302,78 @@ int b200moe_gather_sum(const void* rows_bf16, const int32_t* pos, int32_t T, int
 int b200moe_ep_plan(const int32_t* topk_ids, int32_t T, int32_t K, int32_t experts_per_rank, int32_t world,
                     int32_t* pos, int32_t* counts, int32_t* rows, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Dense operators around the layer.  The reference has none of them beyond its dense GEMMs
+ * (tests/contrib/gemm/): they are what a model runs on either side of the MoE operator.
+ * Element types of their activations: */
+#define B200MOE_T_BF16 0
+#define B200MOE_T_FP16 1
+#define B200MOE_T_FP32 2
+#define B200MOE_T_INT8 3
+/* shape of a gate: none, one value per channel [H], per token [T] or per element [T, H] */
+#define B200MOE_GATE_NONE 0
+#define B200MOE_GATE_CHANNEL 1
+#define B200MOE_GATE_TOKEN 2
+#define B200MOE_GATE_FULL 3
+
+/* Rows to 8-bit integers: scale[t] = max(fl32(max_k |x[t,k]| / 127), 2^-100), q = the whole number nearest to x / scale
+ * (ties to even, decided exactly).  A row that holds an infinity or NaN gets scale NaN and q = 0.
+ *   x: bf16, fp16 or fp32 rows, x_stride elements apart, K <= 16384;  q: i8 [T, K];  scale: f32 [T] */
+int b200moe_quantize_int8(const void* x, int64_t x_stride, int32_t T, int32_t K, int32_t dtype, void* q, float* scale,
+                          void* stream);
+
+/* W8A8 linear layer: y[t,n] = (sum_k q[t,k] weight[n,k]) * scale[t] * weight_scale[n] + bias[n], the sum exact in int32,
+ * rounded once to out_dtype (bf16 or fp16).  K a multiple of 16 below 2^17 (up to 16384 for rows quantised here).
+ *   x          i8 [T, K] (x_dtype INT8, x_stride = K, with x_scale [T]) or bf16 / fp16 / fp32 rows, which are quantised
+ *              first into workspace (round_up(T*K, 256) + 4 T bytes, 16-byte aligned; unused for INT8)
+ *   weight     i8 [N, K], 16-byte aligned;  weight_scale f32 [N];  bias f32 [N] or NULL
+ *   variant    0 = by size, 1 = split-K tiles for few tokens, 2 = CTA pairs
+ *   status     i32 [2] or NULL: word 0 = id of a bounded wait that ran out (left alone otherwise), word 1 = CTA */
+int b200moe_linear_int8(const void* x, int64_t x_stride, int32_t x_dtype, const float* x_scale, const void* weight,
+                        const float* weight_scale, const float* bias, int32_t T, int32_t N, int32_t K, int32_t out_dtype,
+                        int32_t variant, void* workspace, int64_t workspace_bytes, int32_t* status, void* y, void* stream);
+
+/* RMS norms after and before a block, fused with the branch's gate and the residual:
+ *   u = y * rstd(y) * weight (u = y without weight);  h = residual_scale * residual + gate * u;  n = h * rstd(h) * next_weight
+ *   rstd(v) = 1 / sqrt(mean(v^2) + eps).  32-bit arithmetic from the inputs, each output rounded once.  H <= 16384.
+ *   residual, weight, gate, next_weight, h, n may be NULL; rows of y, residual and gate (kind FULL) are *_stride elements apart
+ *   fp32_params: bit 0 weight, bit 1 gate, bit 2 next_weight are fp32 (otherwise of the rows' type)
+ *   q, q_scale: the row that n would be (h without next_weight) as 8-bit integers, as b200moe_quantize_int8 does
+ *   rstd: f32 [2, T] or NULL: rstd(y) and rstd(h), for the backward pass */
+int b200moe_block_norm(const void* y, int64_t y_stride, const void* residual, int64_t residual_stride, const void* weight,
+                       const void* gate, int64_t gate_stride, const void* next_weight, int32_t T, int32_t H, int32_t dtype,
+                       int32_t fp32_params, int32_t gate_kind, float residual_scale, float eps, void* h, void* n, void* q,
+                       float* q_scale, float* rstd, void* stream);
+/* Gradients of the same: dh, dn (contiguous, either may be NULL) -> dy, dresidual, dweight, dgate, dnext_weight in the types of
+ * the tensors they belong to, each NULL where it is not wanted.  Sums over tokens are made in a fixed order. */
+int b200moe_block_norm_bwd_workspace(int32_t T, int32_t H, int32_t dtype, int64_t* bytes);
+int b200moe_block_norm_bwd(const void* y, int64_t y_stride, const void* residual, int64_t residual_stride, const void* weight,
+                           const void* gate, int64_t gate_stride, const void* next_weight, int32_t T, int32_t H, int32_t dtype,
+                           int32_t fp32_params, int32_t gate_kind, float residual_scale, const float* rstd, const void* dh,
+                           const void* dn, void* dy, void* dresidual, void* dweight, void* dgate, void* dnext_weight,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Router with counts and losses; gradients by b200moe_router_backward.  E <= 1024, K <= 32.
+ *   logits bf16 / fp16 / fp32 [T, E], rows `stride` elements apart; scoring and renormalize as in b200moe_route_topk, the K
+ *   experts by descending LOGIT, equal ones in ascending order
+ *   token_mask u8 [T] or NULL (all);  cu_seqlens i32 [sequences + 1] or NULL (one sequence of all tokens): token t belongs to
+ *   sequence s if cu[s] <= t < cu[s+1].  A token that is masked, in no sequence, or whose logits are all -inf counts for
+ *   nothing: ids 0..K-1, weights 0, gradient 0.
+ *   counts i32 [sequences, E];  balance_loss = mean over sequences with n_s > 0 of E / (K n_s^2) sum_e counts sum_t p[t,e],
+ *   p = softmax(logits) or sigmoid(logits) / their sum;  z_loss = mean over live tokens of logsumexp(logits)^2
+ *   lse f32 [2, T], seg i32 [T], coef f32 [sequences, E], stats f32 [2]: for the backward pass, or all NULL */
+int b200moe_router_workspace(int32_t T, int32_t E, int32_t sequences, int64_t* bytes);
+int b200moe_router_forward(const void* logits, int64_t stride, int32_t T, int32_t E, int32_t K, int32_t dtype, int32_t scoring,
+                           int32_t renormalize, const void* token_mask, const int32_t* cu_seqlens, int32_t sequences,
+                           float* topk_weight, int32_t* topk_ids, int32_t* counts, float* balance_loss, float* z_loss, float* lse,
+                           int32_t* seg, float* coef, float* stats, void* workspace, int64_t workspace_bytes, void* stream);
+/* dlogits [T, E] (contiguous, of the logits' type) from the gradients of the weights [T, K], of the balance loss and of the
+ * z-loss (device scalars), each NULL where there is none. */
+int b200moe_router_backward(const void* logits, int64_t stride, int32_t T, int32_t E, int32_t K, int32_t dtype, int32_t scoring,
+                            int32_t renormalize, const float* lse, const int32_t* seg, const float* coef, const float* stats,
+                            const int32_t* topk_ids, const float* topk_weight, const float* dweight, const float* dbalance,
+                            const float* dz, void* dlogits, void* stream);
+
 /* Hardware known-answer probes used by the GPU test-suite and the benchmark (bounded waits).
  *   which = 1: TMA load of one 128-row x 256-element packed-FP4 tile (128-byte swizzle) from `in`
  *              (16384 bytes) -> `out` receives the 16384-byte shared-memory image.

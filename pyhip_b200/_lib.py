@@ -19,7 +19,7 @@ PKG_DIR = pathlib.Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libb200moe.so"
 SOURCES = ["api.cu", "moe_aux.cu", "moe_gemm_sm100.cu", "moe_gemm_fp8_sm100.cu", "moe_gemm_bf16_sm100.cu",
-           "moe_batch1.cu", "forward_static.cu"]
+           "moe_batch1.cu", "forward_static.cu", "block_norm.cu", "router_train.cu", "linear_int8_sm100.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-shared", "-Xcompiler", "-fPIC"]
 
@@ -28,6 +28,8 @@ ACT_SILU, ACT_SWIGLU = 0, 1
 COMBINE_GATHER, COMBINE_FUSED = 0, 1
 ACTQ_TERMS, ACTQ_1X128 = 0, 1
 ABI_VERSION = 3
+T_BF16, T_FP16, T_FP32, T_INT8 = 0, 1, 2, 3
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
 
 
 class Shape(ctypes.Structure):
@@ -61,7 +63,10 @@ EXPORTS = ["b200moe_version", "b200moe_last_error", "b200moe_workspace_layout",
            "b200moe_forward", "b200moe_forward_dyn", "b200moe_sort_align_dyn", "b200moe_sort_align_ws",
            "b200moe_sort_scratch_bytes", "b200moe_route_topk", "b200moe_forward_static", "b200moe_gather_sum", "b200moe_debug_probe",
            "b200moe_forward_ex", "b200moe_static_status", "b200moe_ep_plan", "b200moe_quant_rows_fp8_1x128",
-           "b200moe_forward_batch1", "b200moe_batch1_scratch_bytes"]
+           "b200moe_forward_batch1", "b200moe_batch1_scratch_bytes",
+           "b200moe_quantize_int8", "b200moe_linear_int8", "b200moe_block_norm", "b200moe_block_norm_bwd",
+           "b200moe_block_norm_bwd_workspace", "b200moe_router_workspace", "b200moe_router_forward",
+           "b200moe_router_backward"]
 
 
 def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
@@ -116,6 +121,16 @@ def lib() -> ctypes.CDLL:
     L.b200moe_gather_sum.argtypes = [vp, vp, i32, i32, i32, vp, vp]
     L.b200moe_ep_plan.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp, vp]
     L.b200moe_debug_probe.argtypes = [ctypes.c_int, vp, vp, vp]
+    f32 = ctypes.c_float
+    norm = [vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, i32, i32, i32, f32]
+    L.b200moe_quantize_int8.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp]
+    L.b200moe_linear_int8.argtypes = [vp, i64, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, vp, vp, vp]
+    L.b200moe_block_norm.argtypes = norm + [f32] + [vp] * 6
+    L.b200moe_block_norm_bwd.argtypes = norm + [vp] * 8 + [vp, i64, vp]
+    L.b200moe_block_norm_bwd_workspace.argtypes = [i32, i32, i32, ctypes.POINTER(i64)]
+    L.b200moe_router_workspace.argtypes = [i32, i32, i32, ctypes.POINTER(i64)]
+    L.b200moe_router_forward.argtypes = [vp, i64] + [i32] * 6 + [vp, vp, i32] + [vp] * 10 + [i64, vp]
+    L.b200moe_router_backward.argtypes = [vp, i64] + [i32] * 6 + [vp] * 11
     for name in EXPORTS:
         if name not in ("b200moe_version", "b200moe_last_error"):
             getattr(L, name).restype = ctypes.c_int

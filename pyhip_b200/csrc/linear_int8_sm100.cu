@@ -1,0 +1,605 @@
+// W8A8 linear layer: y[t, n] = (sum_k q[t, k] W[n, k]) * s_t * w_n (+ b_n), 8-bit integers with one fp32 scale per token
+// and per output channel.  tcgen05.mma kind::i8, int32 accumulators in tensor memory: the sum is exact (K < 2^17), so
+// splitting K over CTAs changes no bit of the result.
+//
+// Two kernels, chosen by size (pick_variant):
+//   split   one 128-feature x BT-token tile per CTA, the weights on the MMA's M side; the CTAs of a cluster take equal
+//           ranges of K and add their tiles through distributed shared memory.  For few tokens, where the weights' bytes
+//           and the launch latency bound the call: every weight byte is requested as soon as the CTA starts.
+//   pair    persistent CTA pairs (cta_group::2), 256 tokens x BN features a tile: each CTA holds its 128 tokens' rows and
+//           half of the feature rows, two accumulators overlap a tile's epilogue with the next one's products.
+//
+// A pipeline stage is 128 bytes of K (one swizzle span): 128 rows of one operand and BT or BN/2 rows of the other, one TMA
+// copy each; K and row tails are zero-filled by the copy.  Every barrier wait is bounded; one that runs out sets status[]
+// and the CTA unwinds and frees its tensor memory.
+#include <string.h>
+
+#include <algorithm>
+
+#include "gemm_common.cuh"
+#include "rowwise.cuh"
+
+namespace b200moe {
+
+namespace {
+
+constexpr int kThreadsI8 = 192;                 // warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 epilogue
+constexpr int kTileKI8 = 128;                   // bytes of K per stage
+constexpr int kRowTile = 128;                   // rows of the M-side operand per CTA
+constexpr int kRowTileBytes = kRowTile * kTileKI8;
+constexpr int kMaxStagesI8 = 12;
+constexpr int kSmemLimitI8 = 232448;            // 227 KB
+constexpr int kCtlBytes = 1024;
+constexpr int kStoreCols = 64;                  // columns of a staged store: 128 bytes of a 16-bit type
+constexpr int kPairScaleBytes = 2 * 2 * 256 * 4;   // two tiles' channel scales and biases
+
+struct LinearParams {
+  CUtensorMap tmX;      // token rows (K, T)
+  CUtensorMap tmW;      // weight rows (K, N)
+  CUtensorMap tmY;      // output (N, T), box 64 x 32; only when store_tma
+  const float* x_scale;
+  const float* w_scale;
+  const float* bias;
+  void* y;
+  int32_t* status;
+  int T, N, KB, k_tail_steps, stages, fp16, store_tma, early_weights;
+  int tokens, splits;             // split: token tile, CTAs that share K
+  int m_tiles, n_tiles;           // pair
+};
+
+struct SmemCtlI8 {
+  uint64_t full[kMaxStagesI8];
+  uint64_t empty[kMaxStagesI8];
+  uint64_t tmem_full[2];
+  uint64_t tmem_empty[2];
+  uint32_t tmem_base;
+  uint32_t abort_word;
+};
+static_assert(sizeof(SmemCtlI8) <= kCtlBytes, "control block");
+
+// Instruction descriptor of kind::i8: [4,6) D format (2 = s32)  [7,10) A format  [10,13) B format (1 = signed 8-bit)
+// [17,23) N>>3  [24,29) M>>4; both operands K-major
+__device__ __forceinline__ uint32_t make_idesc_i8(uint32_t M, uint32_t N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+// D[tmem] (+)= A[smem] * B[smem]^T, signed 8-bit x signed 8-bit, K = 32 per instruction
+template <bool PAIR>
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+// into this CTA's shared memory, completing bytes on the pair's leading CTA's barrier
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar & kLeaderMask), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(c0),
+               "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ int4 ld_peer_v4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, bool fp16) {
+  if (fp16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// let this CTA's copies still in flight land before shared memory is released (bounded)
+__device__ __forceinline__ void drain_copies(SmemCtlI8* ctl, int64_t issued, int S) {
+  for (int64_t i = issued > S ? issued - S : 0; i < issued; ++i) {
+    const uint32_t bar = smem_u32(&ctl->full[i % S]);
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_try_wait(bar, (uint32_t)((i / S) & 1)) && global_timer_ns() - t0 < 200000000ull) {}
+  }
+}
+
+// ------------------------------------------------------------------------------------ split
+__global__ void __launch_bounds__(kThreadsI8)
+linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  SmemCtlI8* ctl = reinterpret_cast<SmemCtlI8*>(smem);
+  const uint32_t stage0 = smem_u32(smem) + kCtlBytes;
+  const int S = p.stages, BT = p.tokens, C = p.splits;
+  const uint32_t stage_bytes = (uint32_t)(kRowTileBytes + BT * kTileKI8);
+  const uint32_t cols = (uint32_t)max(32, BT);             // BT is 16 or a power of two from 32 to 256
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)(blockIdx.x % (unsigned)C);        // clusters run along x
+  const int n0 = (int)(blockIdx.x / (unsigned)C) * kRowTile, t0 = (int)blockIdx.y * BT;
+  const int kb0 = (int)((int64_t)p.KB * rank / C), kb1 = (int)((int64_t)p.KB * (rank + 1) / C);
+  volatile uint32_t* abort_word = &ctl->abort_word;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(smem_u32(&ctl->full[s]), 1);
+      mbar_init(smem_u32(&ctl->empty[s]), 1);
+    }
+    mbar_init(smem_u32(&ctl->tmem_full[0]), 1);
+    ctl->abort_word = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&ctl->tmem_base), cols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = ctl->tmem_base;
+
+  bool ok = true;
+  if (warp == 0) {
+    if (lane == 0) {
+      // The weights do not depend on the launch in front when that is this call's own quantiser (early_weights): it
+      // lets this grid start only after everything before it has completed.
+      int ahead = 0;
+      if (p.early_weights)
+        for (; ahead < min(S, kb1 - kb0); ++ahead) {
+          const uint32_t full = smem_u32(&ctl->full[ahead]);
+          mbar_expect_tx(full, stage_bytes);
+          tma_load_2d(stage0 + ahead * stage_bytes, &p.tmW, full, (kb0 + ahead) * kTileKI8, n0);
+        }
+      grid_dep_wait();
+      int64_t issued = 0;
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1, abort_word, 0x1100 + stage)) { ok = false; break; }
+        const uint32_t st = stage0 + stage * stage_bytes, full = smem_u32(&ctl->full[stage]);
+        if (kb - kb0 >= ahead) {
+          mbar_expect_tx(full, stage_bytes);
+          tma_load_2d(st, &p.tmW, full, kb * kTileKI8, n0);
+        }
+        tma_load_2d(st + kRowTileBytes, &p.tmX, full, kb * kTileKI8, t0);
+        ++issued;
+        if (++stage == S) { stage = 0; phase ^= 1; }
+      }
+      if (!ok || *abort_word) drain_copies(ctl, issued, S);
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = make_idesc_i8(kRowTile, (uint32_t)BT);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_word, 0x1200 + stage)) { ok = false; break; }
+      tc_fence_after_sync();
+      __syncwarp();
+      if (elect_one()) {
+        const uint32_t st = stage0 + stage * stage_bytes;
+        const uint32_t a_lo = desc_lo_sw(st), b_lo = desc_lo_sw(st + kRowTileBytes);
+        const int steps = kb == p.KB - 1 ? p.k_tail_steps : 4;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          if (s < steps) umma_i8<false>(tmem_base, a_lo + 2 * s, b_lo + 2 * s, idesc, (kb != kb0 || s != 0) ? 1u : 0u);
+        tc_commit(smem_u32(&ctl->empty[stage]));
+        if (kb == kb1 - 1) tc_commit(smem_u32(&ctl->tmem_full[0]));
+      }
+      __syncwarp();
+      if (++stage == S) { stage = 0; phase ^= 1; }
+    }
+    grid_dep_wait();
+  } else {
+    grid_dep_wait();
+  }
+  grid_dep_launch();
+
+  // the tile as [token][feature] int32 in the stages' memory, which the products no longer need
+  const int live = min(BT, p.T - t0);
+  if (warp >= 2) {
+    ok = mbar_wait(smem_u32(&ctl->tmem_full[0]), 0, abort_word, 0x1300);
+    if (ok) {
+      tc_fence_after_sync();
+      const int quad = warp & 3;
+      const uint32_t at = stage0 + (uint32_t)(quad * 32 + lane) * 4;
+      for (int c0 = 0; c0 < live; c0 += 16) {
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(tmem_base + ((uint32_t)(quad * 32) << 16) + c0, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st_shared_u32(at + (uint32_t)(c0 + i) * (kRowTile * 4), v[i]);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  // token columns are dealt out over the cluster's warps; a lane adds four neighbouring features of all its CTAs
+  const int n = n0 + lane * 4;
+  float ws[4], bs[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    ws[j] = n + j < p.N ? p.w_scale[n + j] : 0.f;
+    bs[j] = (p.bias != nullptr && n + j < p.N) ? p.bias[n + j] : 0.f;
+  }
+  for (int c = rank + C * warp; c < live; c += C * (kThreadsI8 / 32)) {
+    int4 a = make_int4(0, 0, 0, 0);
+    const uint32_t at = stage0 + (uint32_t)c * (kRowTile * 4) + lane * 16;
+#pragma unroll 8
+    for (int r = 0; r < C; ++r) {
+      const int4 v = ld_peer_v4(peer_smem(at, (uint32_t)r));
+      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+    }
+    const float xs = p.x_scale[t0 + c];
+    const float o0 = fmaf((float)a.x * xs, ws[0], bs[0]), o1 = fmaf((float)a.y * xs, ws[1], bs[1]);
+    const float o2 = fmaf((float)a.z * xs, ws[2], bs[2]), o3 = fmaf((float)a.w * xs, ws[3], bs[3]);
+    const uint32_t lo = pack2(o0, o1, p.fp16), hi = pack2(o2, o3, p.fp16);
+    uint16_t* dst = static_cast<uint16_t*>(p.y) + (int64_t)(t0 + c) * p.N + n;
+    if ((p.N & 3) == 0) {
+      if (n < p.N) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+    } else {
+      if (n < p.N) dst[0] = (uint16_t)lo;
+      if (n + 1 < p.N) dst[1] = (uint16_t)(lo >> 16);
+      if (n + 2 < p.N) dst[2] = (uint16_t)hi;
+      if (n + 3 < p.N) dst[3] = (uint16_t)(hi >> 16);
+    }
+  }
+  if (threadIdx.x == 0 && ctl->abort_word != 0 && p.status != nullptr) {
+    p.status[0] = (int32_t)ctl->abort_word;
+    p.status[1] = (int32_t)blockIdx.x;
+  }
+  __syncwarp();
+  cluster_sync_all();                // no CTA leaves while another one reads its tile
+  if (warp == 1) tmem_dealloc(tmem_base, cols);
+}
+
+// ------------------------------------------------------------------------------------ pair
+// tile order: bands of eight token tiles, features running slowest inside a band, so that the CTAs at work at a time share
+// both operands' rows in L2
+__device__ __forceinline__ void tile_of(int w, int m_tiles, int n_tiles, int& m, int& n) {
+  constexpr int BAND = 8;
+  const int band = w / (BAND * n_tiles), first = band * BAND;
+  const int height = min(BAND, m_tiles - first);
+  const int in = w - first * n_tiles;
+  m = first + in % height;
+  n = in / height;
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kThreadsI8, 1)
+linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
+  constexpr uint32_t B_BYTES = BN / 2 * kTileKI8, STAGE = kRowTileBytes + B_BYTES;
+  constexpr uint32_t COLS = 2 * BN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  SmemCtlI8* ctl = reinterpret_cast<SmemCtlI8*>(smem);
+  const int S = p.stages;
+  const uint32_t stage0 = smem_u32(smem) + kCtlBytes;
+  const uint32_t staging = stage0 + S * STAGE;                                    // 4 KB for each epilogue warp
+  float* scales = reinterpret_cast<float*>(smem + kCtlBytes + S * STAGE + 4 * 4096);   // [2][2][BN]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_cta_rank();
+  volatile uint32_t* abort_word = &ctl->abort_word;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(smem_u32(&ctl->full[s]), 1);
+      mbar_init(smem_u32(&ctl->empty[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&ctl->tmem_full[a]), 1);
+      mbar_init(smem_u32(&ctl->tmem_empty[a]), 8);          // the epilogue warps of both CTAs
+    }
+    ctl->abort_word = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&ctl->tmem_base), COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();                  // the partner's barriers exist before anything arrives on them
+  tc_fence_after_sync();
+  const uint32_t tmem_base = ctl->tmem_base;
+  grid_dep_wait();
+  grid_dep_launch();
+
+  const int total = p.m_tiles * p.n_tiles, first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tensormap(&p.tmX);
+      prefetch_tensormap(&p.tmW);
+      int stage = 0;
+      uint32_t phase = 0;
+      int64_t issued = 0;
+      bool ok = true;
+      for (int w = first; w < total && ok; w += step) {
+        int m, n;
+        tile_of(w, p.m_tiles, p.n_tiles, m, n);
+        const int t0 = m * 256 + (int)rank * 128, n0 = n * BN + (int)rank * (BN / 2);
+        for (int kb = 0; kb < p.KB; ++kb) {
+          if (!mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1, abort_word, 0x2100 + stage)) { ok = false; break; }
+          const uint32_t st = stage0 + stage * STAGE, full = smem_u32(&ctl->full[stage]);
+          if (rank == 0) mbar_expect_tx(full, 2 * STAGE);
+          tma_load_2d_pair(st, &p.tmX, full, kb * kTileKI8, t0);
+          tma_load_2d_pair(st + kRowTileBytes, &p.tmW, full, kb * kTileKI8, n0);
+          ++issued;
+          if (++stage == S) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (rank == 0 && (!ok || *abort_word)) drain_copies(ctl, issued, S);
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = make_idesc_i8(256, BN);
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int w = rank == 0 ? first : total; w < total && ok; w += step) {
+      if (!mbar_wait(smem_u32(&ctl->tmem_empty[acc]), acc_phase ^ 1, abort_word, 0x2200 + acc)) break;
+      tc_fence_after_sync();
+      for (int kb = 0; kb < p.KB; ++kb) {
+        if (!mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_word, 0x2300 + stage)) { ok = false; break; }
+        tc_fence_after_sync();
+        __syncwarp();
+        if (elect_one()) {
+          const uint32_t st = stage0 + stage * STAGE;
+          const uint32_t a_lo = desc_lo_sw(st), b_lo = desc_lo_sw(st + kRowTileBytes);
+          const int steps = kb == p.KB - 1 ? p.k_tail_steps : 4;
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            if (s < steps) umma_i8<true>(tmem_base + acc * BN, a_lo + 2 * s, b_lo + 2 * s, idesc, (kb != 0 || s != 0) ? 1u : 0u);
+          tc_commit_pair(smem_u32(&ctl->empty[stage]));
+          if (kb == p.KB - 1) tc_commit_pair(smem_u32(&ctl->tmem_full[acc]));
+        }
+        __syncwarp();
+        if (++stage == S) { stage = 0; phase ^= 1; }
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+  } else {
+    const int quad = warp & 3, te = threadIdx.x - 64;
+    const uint32_t mine = staging + (uint32_t)(warp - 2) * 4096;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int w = first; w < total; w += step) {
+      int m, n;
+      tile_of(w, p.m_tiles, p.n_tiles, m, n);
+      const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * BN;
+      float* sc = scales + acc * 2 * BN;
+      for (int i = te; i < BN; i += 128) {
+        const bool in = n0 + i < p.N;
+        sc[i] = in ? p.w_scale[n0 + i] : 0.f;
+        sc[BN + i] = (in && p.bias != nullptr) ? p.bias[n0 + i] : 0.f;
+      }
+      const float xs = row0 + lane < p.T ? p.x_scale[row0 + lane] : 0.f;
+      const bool ok = mbar_wait(smem_u32(&ctl->tmem_full[acc]), acc_phase, abort_word, 0x2400 + acc);
+      uint32_t all;                        // every epilogue warp of the CTA sees the scales, or all of them give up
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                   : "=r"(all) : "r"((uint32_t)ok) : "memory");
+      if (!all) break;
+      tc_fence_after_sync();
+      const uint32_t tacc = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN;
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN; c0 += kStoreCols) {
+        if (row0 >= p.T || n0 + c0 >= p.N) break;
+        if (lane == 0) bulk_wait_read();    // the staging rows' previous copy has been read out
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < kStoreCols; h += 16) {
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(tacc + c0 + h, v);
+          tmem_ld_wait();
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const float4 ws = *reinterpret_cast<const float4*>(sc + c0 + h + i);
+            const float4 bs = *reinterpret_cast<const float4*>(sc + BN + c0 + h + i);
+            o[i / 2] = pack2(fmaf((float)(int)v[i] * xs, ws.x, bs.x), fmaf((float)(int)v[i + 1] * xs, ws.y, bs.y), p.fp16);
+            o[i / 2 + 1] = pack2(fmaf((float)(int)v[i + 2] * xs, ws.z, bs.z), fmaf((float)(int)v[i + 3] * xs, ws.w, bs.w), p.fp16);
+          }
+          const uint32_t row = mine + (uint32_t)lane * 128;
+          const uint32_t j = (uint32_t)h / 8;
+          st_shared_v4(row + ((j ^ (lane & 7)) << 4), o[0], o[1], o[2], o[3]);
+          st_shared_v4(row + (((j + 1) ^ (lane & 7)) << 4), o[4], o[5], o[6], o[7]);
+        }
+        if (p.store_tma) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&p.tmY, mine, n0 + c0, row0);
+            bulk_commit();
+          }
+        } else {
+          // rows of y that do not start on 16 bytes: a row at a time, two neighbouring values a lane
+          __syncwarp();
+          const int col = n0 + c0 + lane * 2;
+          for (int r = 0; r < 32 && row0 + r < p.T; ++r) {
+            uint32_t v;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(mine + (uint32_t)r * 128 + ((((uint32_t)lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4));
+            uint16_t* dst = static_cast<uint16_t*>(p.y) + (int64_t)(row0 + r) * p.N + col;
+            if (col < p.N) dst[0] = (uint16_t)v;
+            if (col + 1 < p.N) dst[1] = (uint16_t)(v >> 16);
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_leader(smem_u32(&ctl->tmem_empty[acc]));
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (threadIdx.x == 0 && ctl->abort_word != 0 && p.status != nullptr) {
+    p.status[0] = (int32_t)ctl->abort_word;
+    p.status[1] = (int32_t)blockIdx.x;
+  }
+  cluster_sync_all();     // neither CTA leaves while the other's products or arrivals may still touch it
+  if (warp == 1) tmem_dealloc_pair(tmem_base, COLS);
+}
+
+// ------------------------------------------------------------------------------------ host
+int encode_rows(CUtensorMap* map, const void* base, int K, int rows, int box_rows, const char* what) {
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)K};
+  cuuint32_t box[2] = {kTileKI8, (cuuint32_t)box_rows};
+  return encode_map_sw(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, what);
+}
+
+struct Variant {
+  bool pair;
+  int tokens, splits, stages;    // split
+  int bn;                        // pair
+};
+
+Variant pick_variant(int T, int N, int KB, int force) {
+  Variant v = {};
+  const int sms = device_sm_count();
+  v.pair = force == 2 || (force == 0 && T > 256);
+  if (v.pair) {
+    const int64_t tiles = (int64_t)((T + 255) / 256) * ((N + 255) / 256);
+    v.bn = tiles * 2 >= sms ? 256 : 128;
+    return v;
+  }
+  v.tokens = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  const int64_t tiles = (int64_t)((N + kRowTile - 1) / kRowTile) * ((T + v.tokens - 1) / v.tokens);
+  v.splits = 1;
+  while (v.splits < 8 && tiles * v.splits * 2 <= 3 * sms && KB / (v.splits * 2) >= 2) v.splits *= 2;
+  const int stage = kRowTileBytes + v.tokens * kTileKI8;
+  const int kb = (KB + v.splits - 1) / v.splits;
+  v.stages = std::min({kb, kMaxStagesI8, 110 * 1024 / stage});
+  return v;
+}
+
+}  // namespace
+
+int launch_linear_int8(const void* q, const float* x_scale, const void* w, const float* w_scale, const float* bias, void* y, int T,
+                       int N, int K, int fp16, int early_weights, int variant, int32_t* status, cudaStream_t st) {
+  LinearParams p;
+  memset(&p, 0, sizeof(p));
+  p.KB = (K + kTileKI8 - 1) / kTileKI8;
+  p.k_tail_steps = (K - (p.KB - 1) * kTileKI8 + 31) / 32;
+  p.T = T; p.N = N; p.x_scale = x_scale; p.w_scale = w_scale; p.bias = bias; p.y = y; p.status = status; p.fp16 = fp16;
+  const Variant v = pick_variant(T, N, p.KB, variant);
+  if (!v.pair) {
+    p.tokens = v.tokens; p.splits = v.splits; p.stages = v.stages; p.early_weights = early_weights;
+    if (int rc = encode_rows(&p.tmX, q, K, T, v.tokens, "int8 token rows")) return rc;
+    if (int rc = encode_rows(&p.tmW, w, K, N, kRowTile, "int8 weights")) return rc;
+    const int n_tiles = (N + kRowTile - 1) / kRowTile, t_tiles = (T + v.tokens - 1) / v.tokens;
+    B200_CHECK_ARG(t_tiles <= 65535, "linear_int8: %d tokens", T);
+    const int stage = kRowTileBytes + v.tokens * kTileKI8;
+    // At least the share of shared memory that its columns are of tensor memory: CTAs that fit an SM's shared memory
+    // then fit its tensor memory too, and no cluster waits for columns that another waiting cluster holds.
+    const int share = (int)((int64_t)kSmemLimitI8 * std::max(32, v.tokens) / 512);
+    const int bytes = std::max({v.stages * stage, std::min(v.tokens, T) * kRowTile * 4 + 16 * kRowTile * 4, share});
+    const size_t smem = 1024 + kCtlBytes + (size_t)bytes;
+    B200_CHECK_CUDA(cudaFuncSetAttribute(linear_int8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimitI8));
+    B200_CHECK_CUDA(launch_chained_cluster(linear_int8_split_kernel, dim3(n_tiles * v.splits, t_tiles), dim3(kThreadsI8), smem, st,
+                                           v.splits, p));
+    return 0;
+  }
+  const int bn = v.bn;
+  p.m_tiles = (T + 255) / 256;
+  p.n_tiles = (N + bn - 1) / bn;
+  if (int rc = encode_rows(&p.tmX, q, K, T, 128, "int8 token rows")) return rc;
+  if (int rc = encode_rows(&p.tmW, w, K, N, bn / 2, "int8 weights")) return rc;
+  p.store_tma = N % 8 == 0 && ((uintptr_t)y & 15) == 0;
+  if (p.store_tma) {
+    cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)T};
+    cuuint64_t strides[1] = {(cuuint64_t)N * 2};
+    cuuint32_t box[2] = {kStoreCols, 32};
+    if (int rc = encode_map_sw(&p.tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_NONE, "linear output"))
+      return rc;
+  }
+  const int stage = kRowTileBytes + bn / 2 * kTileKI8;
+  p.stages = std::min((kSmemLimitI8 - 1024 - kCtlBytes - 4 * 4096 - kPairScaleBytes) / stage, kMaxStagesI8);
+  const size_t smem = 1024 + kCtlBytes + (size_t)p.stages * stage + 4 * 4096 + kPairScaleBytes;
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  B200_CHECK_ARG(tiles < (1ll << 30), "linear_int8: T=%d N=%d", T, N);
+  const int grid = 2 * (int)std::min<int64_t>(device_sm_count() / 2, tiles);
+  void (*k)(LinearParams) = bn == 256 ? linear_int8_pair_kernel<256> : linear_int8_pair_kernel<128>;
+  B200_CHECK_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimitI8));
+  B200_CHECK_CUDA(launch_chained_cluster(k, dim3(grid), dim3(kThreadsI8), smem, st, 2, p));
+  return 0;
+}
+
+}  // namespace b200moe
+
+using namespace b200moe;
+
+extern "C" int b200moe_linear_int8(const void* x, int64_t x_stride, int32_t x_dtype, const float* x_scale, const void* weight,
+                                   const float* weight_scale, const float* bias, int32_t T, int32_t N, int32_t K, int32_t out_dtype,
+                                   int32_t variant, void* workspace, int64_t workspace_bytes, int32_t* status, void* y, void* stream) {
+  B200_CHECK_ARG(T >= 0 && N >= 1 && K >= 16 && K % 16 == 0 && K < (1 << 17), "linear_int8: T=%d N=%d K=%d (K a multiple of 16 below 2^17)",
+                 T, N, K);
+  B200_CHECK_ARG(out_dtype == B200MOE_T_BF16 || out_dtype == B200MOE_T_FP16, "linear_int8: out dtype %d", out_dtype);
+  B200_CHECK_ARG(x_dtype == B200MOE_T_INT8 || (x_dtype >= B200MOE_T_BF16 && x_dtype <= B200MOE_T_FP32), "linear_int8: x dtype %d", x_dtype);
+  B200_CHECK_ARG(variant >= 0 && variant <= 2, "linear_int8: variant %d", variant);
+  if (T == 0) return 0;
+  B200_CHECK_ARG(x && weight && weight_scale && y, "linear_int8: NULL pointer");
+  B200_CHECK_ARG(((uintptr_t)weight & 15) == 0, "linear_int8: weight must be 16-byte aligned");
+  B200_CHECK_ARG(((uintptr_t)y & 7) == 0, "linear_int8: y must be 8-byte aligned");
+  cudaStream_t st = (cudaStream_t)stream;
+  const void* q = x;
+  const float* scale = x_scale;
+  if (x_dtype != B200MOE_T_INT8) {
+    // the quantised rows and their scales
+    const int64_t rows = round_up64((int64_t)T * K, 256);
+    B200_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= rows + (int64_t)T * 4,
+                   "linear_int8: workspace holds %lld bytes of %lld", (long long)workspace_bytes, (long long)(rows + (int64_t)T * 4));
+    q = workspace;
+    scale = (const float*)((uint8_t*)workspace + rows);
+    if (int rc = b200moe_quantize_int8(x, x_stride, T, K, x_dtype, workspace, const_cast<float*>(scale), stream)) return rc;
+  } else {
+    B200_CHECK_ARG(x_scale != nullptr && x_stride == K && ((uintptr_t)x & 15) == 0, "linear_int8: 8-bit rows must be contiguous, 16-byte aligned and have x_scale");
+  }
+  return launch_linear_int8(q, scale, weight, weight_scale, bias, y, T, N, K, out_dtype == B200MOE_T_FP16, x_dtype != B200MOE_T_INT8, variant,
+                            status, st);
+}

@@ -1,4 +1,4 @@
-"""Dense block-scaled linear layers on the MoE main loop.
+"""Dense linear layers: block-scaled ones on the MoE main loop, and the W8A8 layer with kernels of its own.
 
 The reference carries separate dense kernels for the projections either side of the MoE layer
 (src/contrib/gemm_a4w4.py driven by tests/contrib/gemm/test_a4w4_mxfp4.py:22-58, and the FP8
@@ -7,6 +7,9 @@ block-scale GEMM of tests/contrib/gemm/test_a8w8_f32_blockscale.py:114-191).  He
 expert 0 in token order (the sort is stable), the activation quantiser gathers nothing, and the
 rows the GEMM stores in sorted order are already the result.  Same kernels, same formats, same
 C ABI calls (`b200moe_sort_align`, `b200moe_quant_rows[_e4m3]`, `b200moe_down`).
+
+`linear_int8` is the product of 8-bit integers with one scale per token and per output channel, which the reference does not
+have: its C ABI call (`b200moe_linear_int8`) quantises the tokens and multiplies, two launches.
 """
 from __future__ import annotations
 
@@ -16,6 +19,7 @@ import torch
 
 from . import _lib
 from .fused_moe import _capacity, _ptr, _stream, get_plan, pick_block
+from .rows import MAX_ROW, ROW_TYPES, on_device, rows_of, stream_of
 
 
 class PreparedLinear:
@@ -104,3 +108,111 @@ def linear_fp8_128x128(x, weight, weight_scale, block_size_M=None):
     """bf16 x [M, K] times e4m3 weight [N, K] with one fp32 scale per 128x128 block [N/128, K/128]
     -> bf16 [M, N] (the reference's block-scale FP8 GEMM, tests/contrib/gemm/test_a8w8_f32_blockscale.py:114-191)."""
     return _linear(x, weight, weight_scale, _lib.W_FP8_128, 0, block_size_M)
+
+
+def quantize_int8(x):
+    """Rows of bf16, fp16 or fp32 ``x`` [..., K] -> (q int8 [..., K], scale f32 [...]) with
+    scale = max(max |x| / 127, 2**-100) and q the whole number nearest to x / scale (ties to even, decided exactly).
+    The activation format of `linear_int8`; with rows as output channels it also makes that layer's weights.
+    A row that holds an infinity or NaN gets scale NaN.  K <= 16384.  There is no gradient."""
+    if not x.is_cuda:
+        raise RuntimeError("quantize_int8 runs on a CUDA device only (sm_100a); there is no CPU path")
+    dt = ROW_TYPES.get(x.dtype)
+    if dt is None:
+        raise TypeError("x must be bfloat16, float16 or float32")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_ROW:
+        raise ValueError(f"rows of x must have 1 to {MAX_ROW} values")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("quantize_int8 has no gradient: call it under torch.no_grad() or on a detached tensor")
+    with on_device(x):
+        x2, stride = rows_of(x)
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        _lib.check(_lib.lib().b200moe_quantize_int8(x2.data_ptr(), stride, x2.shape[0], x2.shape[1], dt, q.data_ptr(),
+                                                    scale.data_ptr(), stream_of(x)), "quantize_int8")
+    return q, scale
+
+
+_int8_status: dict = {}
+
+
+def int8_status(device=None):
+    """Host read of the error words that `linear_int8` calls on ``device`` leave (synchronises; for tests and debugging):
+    (id of the barrier wait that ran out, its CTA), (0, 0) if none ever did."""
+    t = _int8_status.get(torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device))
+    return (0, 0) if t is None else tuple(t.cpu().tolist())
+
+
+def linear_int8(x, weight, weight_scale, *, x_scale=None, bias=None, out_dtype=None, variant: int = 0):
+    """W8A8 linear layer, y = (q @ weight^T) * scale[token] * weight_scale[channel] (+ bias), the integer sums exact and the
+    result rounded once.
+
+      ``x``: bf16 / fp16 / fp32 [..., K], quantised per token here as `quantize_int8` does (K <= 16384), or int8 [..., K] with
+        ``x_scale`` f32 [...] (from `quantize_int8` or `fused_pre_norm(..., quant="int8")`)
+      ``weight``: int8 [N, K], ``weight_scale``: f32 [N] (for example ``quantize_int8(w)``); used in place, nothing is kept
+      ``bias``: f32 [N]
+      ``out_dtype``: bfloat16 or float16; the default is x's type, bfloat16 for int8 and fp32 rows
+      ``variant``: 0 chooses the kernel by size, 1 = split-K tiles for few tokens, 2 = CTA pairs
+
+    K must be a multiple of 16 below 2**17.  There is no gradient.  Returns [..., N]."""
+    if not x.is_cuda:
+        raise RuntimeError("linear_int8 runs on a CUDA device only (sm_100a); there is no CPU path")
+    dev = x.device
+    if weight.dtype != torch.int8 or weight.dim() != 2:
+        raise TypeError("weight must be an int8 matrix [N, K]")
+    N, K = weight.shape
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"x has shape {tuple(x.shape)}, the weight {K} columns")
+    if N < 1 or K < 16 or K % 16 or K >= 1 << 17:
+        raise ValueError(f"weight [{N}, {K}]: K must be a multiple of 16 below 2**17")
+    if weight_scale.dtype != torch.float32 or weight_scale.numel() != N:
+        raise ValueError("weight_scale must hold one float32 scale per output channel")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != N):
+        raise ValueError("bias must hold one float32 value per output channel")
+    if x.dtype == torch.int8:
+        dt = _lib.T_INT8
+        if x_scale is None or x_scale.dtype != torch.float32 or x_scale.shape != x.shape[:-1]:
+            raise ValueError("int8 rows need x_scale, one float32 per row")
+    else:
+        dt = ROW_TYPES.get(x.dtype)
+        if dt is None:
+            raise TypeError("x must be int8, bfloat16, float16 or float32")
+        if x_scale is not None:
+            raise ValueError("x_scale belongs to int8 rows")
+        if K > MAX_ROW:
+            raise ValueError(f"rows that are quantised here have up to {MAX_ROW} values")
+    for t in (weight, weight_scale, x_scale, bias):
+        if t is not None and t.device != dev:
+            raise ValueError("all tensors must be on one device")
+    if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (x_scale is not None and x_scale.requires_grad)):
+        raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad() or on detached tensors")
+    if out_dtype is None:
+        out_dtype = x.dtype if dt in (_lib.T_BF16, _lib.T_FP16) else torch.bfloat16
+    if out_dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("out_dtype must be bfloat16 or float16")
+    if variant not in (0, 1, 2):
+        raise ValueError(f"variant={variant!r}: 0, 1 or 2")
+    with on_device(x):
+        status = _int8_status.get(dev)
+        if status is None and not torch.cuda.is_current_stream_capturing():     # a graph's own memory would not outlive it
+            status = _int8_status[dev] = torch.zeros(2, dtype=torch.int32, device=dev)
+        x2, stride = rows_of(x)
+        T = x2.shape[0]
+        y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=dev)
+        ws = xs = None
+        need = 0
+        if dt == _lib.T_INT8:
+            if stride != K or x2.data_ptr() & 15:
+                x2, stride = x2.clone(memory_format=torch.contiguous_format), K
+            xs = x_scale.contiguous()
+        else:
+            need = (T * K + 255) // 256 * 256 + 4 * T
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        w = weight if weight.is_contiguous() and not weight.data_ptr() & 15 else weight.clone(memory_format=torch.contiguous_format)
+        sc, b = weight_scale.contiguous(), None if bias is None else bias.contiguous()
+        _lib.check(_lib.lib().b200moe_linear_int8(
+            x2.data_ptr(), stride, dt, None if xs is None else xs.data_ptr(), w.data_ptr(), sc.data_ptr(),
+            None if b is None else b.data_ptr(), T, N, K, ROW_TYPES[out_dtype], variant, None if ws is None else ws.data_ptr(), need,
+            None if status is None else status.data_ptr(), y.data_ptr(), stream_of(x)), "linear_int8")
+    return y
