@@ -21,7 +21,7 @@ LIB_PATH = PKG_DIR / "libb200moe.so"
 SOURCES = ["api.cu", "moe_aux.cu", "moe_gemm_sm100.cu", "moe_gemm_fp8_sm100.cu", "moe_gemm_bf16_sm100.cu",
            "moe_batch1.cu", "forward_static.cu", "block_norm.cu", "router_train.cu", "linear_int8_sm100.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-shared", "-Xcompiler", "-fPIC"]
+              "--threads", "0", "-shared", "-Xcompiler", "-fPIC"]
 
 W_MXFP4, W_FP8_128, W_FP8_ROW, W_BF16 = 0, 1, 2, 3
 ACT_SILU, ACT_SWIGLU = 0, 1

@@ -5,8 +5,11 @@
 // All of it in 32 bits from the inputs, rounded once where it is stored: n is the norm of the unrounded h.
 //
 // Bound by memory: forward reads y and r and writes h and n (8 bytes a value in 16-bit types), backward reads
-// y, r, dh, dn and writes dy and dr (12 bytes).  A row stays in the registers of the threads that share it (each takes
-// the same columns of every row, in 16-byte pieces), so every value is read and written once.
+// y, r, dh, dn and writes dy and dr (12 bytes).  The threads that share a row take the same columns of every row, in
+// 16-byte pieces, so every value is read and written once and the sums over tokens stay in registers.
+// Two forms.  Plain: a row goes straight to registers; any alignment, and the lowest latency for few rows.  Ring: a
+// thread copies its pieces of the next rows to shared memory while it works on the present one (it reads nothing but
+// its own copies, so no barrier), which keeps tens of KB in flight per SM where the plain form waits at every row.
 #include <algorithm>
 
 #include "rowwise.cuh"
@@ -17,6 +20,7 @@ namespace {
 
 constexpr int kRowThreads = 512;          // threads of a CTA at most
 constexpr int kMaxNormWidth = 16384;
+constexpr int kRingLimit = 224 * 1024;    // shared memory of a ring: what an SM has, less the reductions' slots
 template <typename T> constexpr int kMaxPieces = kMaxNormWidth / (16 / (int)sizeof(T)) / kRowThreads;   // 16-byte pieces of a thread
 
 struct NormParams {
@@ -144,6 +148,187 @@ block_norm_kernel(const __grid_constant__ NormParams p) {
   }
 }
 
+// piece c of a gate per channel, which is fp32 or of the rows' type whatever the weights are
+template <typename T, int N2>
+__device__ __forceinline__ void load_gate_piece(const NormParams& p, int c, float2 (&o)[N2]) {
+  if (p.gate_f32) load_piece<T, float>(p.gate, c, o); else load_piece<T, T>(p.gate, c, o);
+}
+
+// Forward over a ring of two rows in shared memory, 16-byte pieces and pairs of values throughout, 16 values to a thread.
+// GATE: 0 none or per token, 1 per channel, 2 per element.  P: type of the norms' weights.
+// HOLD: the weights (times the gate per channel) stay in registers over the rows.  L1 would serve them at every row, which
+// costs it as much as the rows themselves (66 % of its data pipe with fp32 weights; 43.8 -> 36.8 us at 8192 x 2880).  It takes
+// 85 registers, so 768 threads an SM; rows so wide that only one CTA of those would fit read the weights again and have two
+// CTAs of 64 registers (4096 x 7168: 47 against 65 us).
+constexpr int kNormValues = 16;
+constexpr int kHoldThreads = 768, kNoHoldThreads = 1024;      // of an SM
+template <typename T, typename P, bool POST, int GATE, bool HOLD>
+__global__ void __launch_bounds__(HOLD ? kHoldThreads : kNoHoldThreads, 1)
+block_norm_ring_kernel(const __grid_constant__ NormParams p) {
+  constexpr int VEC = 16 / sizeof(T), NV = kNormValues / VEC, N2 = VEC / 2;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ __align__(16) float slots[2 * 3 * 32];
+  CtaReduce red(slots);
+  grid_dep_wait();
+  grid_dep_launch();
+  const int chunks = p.H / VEC, tpr = (int)blockDim.x, tid = (int)threadIdx.x;
+  const bool res = p.r != nullptr, next = p.wn != nullptr;
+  const uint32_t array_bytes = (uint32_t)chunks * 16;
+  const uint32_t at_g = array_bytes * (1 + res), stage_bytes = at_g + (GATE == 2 ? array_bytes : 0);
+  const uint32_t mine = smem_u32(ring) + (uint32_t)tid * 16;
+  const float inv_h = 1.f / (float)p.H;
+  auto fetch = [&](int64_t t, uint32_t at) {
+    if (t < p.T) {
+      const uint4* y = reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + t * p.y_stride) + tid;
+      const uint4* r = reinterpret_cast<const uint4*>(static_cast<const T*>(p.r) + t * p.r_stride) + tid;
+      const uint4* g = reinterpret_cast<const uint4*>(static_cast<const T*>(p.gate) + t * p.gate_stride) + tid;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (tid + i * tpr < chunks) {
+          const uint32_t dst = at + (uint32_t)(i * tpr) * 16;
+          copy16_async(dst, y + i * tpr);
+          if (res) copy16_async(dst + array_bytes, r + i * tpr);
+          if (GATE == 2) copy16_async(dst + at_g, g + i * tpr);
+        }
+      }
+    }
+    copy_commit();
+  };
+  // the factor of y in piece c that the rows share, and the next norm's weights
+  auto load_factor = [&](int c, float2 (&f)[N2]) {
+#pragma unroll
+    for (int j = 0; j < N2; ++j) f[j] = both(1.f);
+    if (POST) load_piece<T, P>(p.w, c, f);
+    if (GATE == 1) {
+      float2 g[N2];
+      load_gate_piece<T>(p, c, g);
+#pragma unroll
+      for (int j = 0; j < N2; ++j) f[j] = mul2(f[j], g[j]);
+    }
+  };
+  const int64_t step = gridDim.x;
+  fetch(blockIdx.x, mine);
+  float2 hold_f[HOLD ? NV : 1][N2], hold_n[HOLD ? NV : 1][N2];
+  if (HOLD) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + i * tpr < chunks) {
+        load_factor(tid + i * tpr, hold_f[i]);
+        if (next) load_piece<T, P>(p.wn, tid + i * tpr, hold_n[i]);
+      }
+  }
+  uint32_t at = mine, other = mine + stage_bytes;
+  for (int64_t t = blockIdx.x; t < p.T; t += step) {
+    copy_wait<0>();
+    fetch(t + step, other);                       // the stage that the row before has left
+    float2 h[NV][N2];
+    float scale = 1.f;                            // rstd(y) and a token's gate
+    if (POST) {
+      float2 ss = both(0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (tid + i * tpr < chunks) {
+          unpack16(lds16(at + (uint32_t)(i * tpr) * 16), h[i], T());
+#pragma unroll
+          for (int j = 0; j < N2; ++j) ss = fma2(h[i][j], h[i][j], ss);
+        }
+      float sum[1] = {ss.x + ss.y};
+      red.sum(sum);
+      scale = rsqrtf(sum[0] * inv_h + p.eps);
+      if (tid == 0 && p.rstd != nullptr) p.rstd[t] = scale;
+    }
+    if (GATE == 0 && p.gate_kind == B200MOE_GATE_TOKEN) {
+      float g1[1];
+      load_param<T, 1>(p.gate, p.gate_f32, t * p.gate_stride, g1);
+      scale *= g1[0];
+    }
+    const float2 scale2 = both(scale), alpha2 = both(p.alpha);
+    float2 ss = both(0.f);
+    uint4* ho = reinterpret_cast<uint4*>(static_cast<T*>(p.h) + t * p.H) + tid;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + i * tpr < chunks) {
+        const uint32_t src = at + (uint32_t)(i * tpr) * 16;
+        float2 f[N2], r[N2];
+        if (!POST) unpack16(lds16(src), h[i], T());
+        if (HOLD) {
+#pragma unroll
+          for (int j = 0; j < N2; ++j) f[j] = hold_f[i][j];
+        } else {
+          load_factor(tid + i * tpr, f);
+        }
+#pragma unroll
+        for (int j = 0; j < N2; ++j) h[i][j] = mul2(h[i][j], (POST || GATE == 1) ? mul2(f[j], scale2) : scale2);
+        if (GATE == 2) {
+          unpack16(lds16(src + at_g), r, T());
+#pragma unroll
+          for (int j = 0; j < N2; ++j) h[i][j] = mul2(h[i][j], r[j]);
+        }
+        if (res) {
+          unpack16(lds16(src + array_bytes), r, T());
+#pragma unroll
+          for (int j = 0; j < N2; ++j) h[i][j] = fma2(r[j], alpha2, h[i][j]);
+        }
+#pragma unroll
+        for (int j = 0; j < N2; ++j) ss = fma2(h[i][j], h[i][j], ss);
+        if (p.h != nullptr) ho[i * tpr] = pack16(h[i], T());
+      }
+    if (next) {
+      float sum[1] = {ss.x + ss.y};
+      red.sum(sum);
+      const float rh = rsqrtf(sum[0] * inv_h + p.eps);
+      if (tid == 0 && p.rstd != nullptr) p.rstd[p.T + t] = rh;
+      const float2 rh2 = both(rh);
+      uint4* no = reinterpret_cast<uint4*>(static_cast<T*>(p.n) + t * p.H) + tid;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (tid + i * tpr < chunks) {
+          float2 f[N2];
+          if (HOLD) {
+#pragma unroll
+            for (int j = 0; j < N2; ++j) f[j] = hold_n[i][j];
+          } else {
+            load_piece<T, P>(p.wn, tid + i * tpr, f);
+          }
+#pragma unroll
+          for (int j = 0; j < N2; ++j) h[i][j] = mul2(h[i][j], mul2(f[j], rh2));
+          if (p.n != nullptr) no[i * tpr] = pack16(h[i], T());
+        }
+    }
+    if (p.q != nullptr) {
+      uint32_t m[1] = {0};
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (tid + i * tpr < chunks) {
+#pragma unroll
+          for (int j = 0; j < N2; ++j)
+            m[0] = max(m[0], max(__float_as_uint(h[i][j].x) & 0x7fffffffu, __float_as_uint(h[i][j].y) & 0x7fffffffu));
+        }
+      red.max_u32(m);
+      const float sc = int8_scale(m[0]);
+      const bool bad = m[0] >= 0x7f800000u;
+      const float inv = __frcp_rn(sc);
+      if (tid == 0) p.q_scale[t] = sc;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = tid + i * tpr;
+        if (c < chunks) {
+          Pack<int8_t, VEC> k;
+#pragma unroll
+          for (int j = 0; j < N2; ++j) {
+            k.v[2 * j] = bad ? (int8_t)0 : (int8_t)quant_int8(h[i][j].x, sc, inv);
+            k.v[2 * j + 1] = bad ? (int8_t)0 : (int8_t)quant_int8(h[i][j].y, sc, inv);
+          }
+          *reinterpret_cast<Pack<int8_t, VEC>*>(p.q + t * p.H + c * VEC) = k;
+        }
+      }
+    }
+    const uint32_t swap = at;
+    at = other;
+    other = swap;
+  }
+}
+
 // Backward.  With e = dh + rstd(h) w' dn and c = rstd(h)^3 mean(w' dn h) the gradient that reaches h is e - c h, and the
 // sum that the norm of y needs, sum(w y g (e - c h)), is A - c B with A = sum(w y g e), B = sum(w y g h): all three sums
 // of a row are formed in one reduction.  A gate per token is a factor of A and B, and its own gradient is rstd(y)(A - cB).
@@ -262,6 +447,198 @@ block_norm_bwd_kernel(const __grid_constant__ NormBwdParams b) {
   }
 }
 
+// Backward over a ring of rows in shared memory.  What a row needs twice (y, dn) is read from there again instead of held,
+// so that 16 values a thread and their sums over tokens fit the registers.  GATE and P as in the forward kernel.
+template <typename T, typename P, int GATE, bool POST, bool NEXT>
+__global__ void __launch_bounds__(kRowThreads, 1)
+block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
+  constexpr int VEC = 16 / sizeof(T), NV = 16 / VEC, N2 = VEC / 2;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ __align__(16) float slots[2 * 3 * 32];
+  const NormParams& p = b.f;
+  CtaReduce red(slots);
+  grid_dep_wait();
+  grid_dep_launch();
+  const int chunks = p.H / VEC, tpr = (int)blockDim.x, tid = (int)threadIdx.x;
+  const bool res = p.r != nullptr, has_dh = b.dh != nullptr, has_dn = NEXT && b.dn != nullptr;
+  const uint32_t array_bytes = (uint32_t)chunks * 16;
+  const uint32_t at_r = array_bytes, at_h = at_r + (res ? array_bytes : 0), at_n = at_h + (has_dh ? array_bytes : 0);
+  const uint32_t at_g = at_n + (has_dn ? array_bytes : 0), stage_bytes = at_g + (GATE == 2 ? array_bytes : 0);
+  const uint32_t mine = smem_u32(ring) + (uint32_t)tid * 16;
+  const float inv_h = 1.f / (float)p.H;
+  const bool token = GATE == 0 && p.gate_kind == B200MOE_GATE_TOKEN;
+  auto fetch = [&](int64_t t, uint32_t at) {
+    if (t < p.T) {
+      const uint4* y = reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + t * p.y_stride) + tid;
+      const uint4* r = reinterpret_cast<const uint4*>(static_cast<const T*>(p.r) + t * p.r_stride) + tid;
+      const uint4* dh = reinterpret_cast<const uint4*>(static_cast<const T*>(b.dh) + t * p.H) + tid;
+      const uint4* dn = reinterpret_cast<const uint4*>(static_cast<const T*>(b.dn) + t * p.H) + tid;
+      const uint4* g = reinterpret_cast<const uint4*>(static_cast<const T*>(p.gate) + t * p.gate_stride) + tid;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (tid + i * tpr < chunks) {
+          const uint32_t dst = at + (uint32_t)(i * tpr) * 16;
+          copy16_async(dst, y + i * tpr);
+          if (res) copy16_async(dst + at_r, r + i * tpr);
+          if (has_dh) copy16_async(dst + at_h, dh + i * tpr);
+          if (has_dn) copy16_async(dst + at_n, dn + i * tpr);
+          if (GATE == 2) copy16_async(dst + at_g, g + i * tpr);
+        }
+      }
+    }
+    copy_commit();
+  };
+  float2 aw[POST ? NV : 1][N2], an[NEXT ? NV : 1][N2], ag[GATE == 1 ? NV : 1][N2];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < N2; ++j) {
+      if (POST) aw[i][j] = both(0.f);
+      if (NEXT) an[i][j] = both(0.f);
+      if (GATE == 1) ag[i][j] = both(0.f);
+    }
+  const int64_t step = gridDim.x;
+  fetch(blockIdx.x, mine);
+  uint32_t at = mine, other = mine + stage_bytes;
+  for (int64_t t = blockIdx.x; t < p.T; t += step) {
+    copy_wait<0>();
+    fetch(t + step, other);                       // the stage that the row before has left
+    float gt = 1.f;
+    if (token) {
+      float g1[1];
+      load_param<T, 1>(p.gate, p.gate_f32, t * p.gate_stride, g1);
+      gt = g1[0];
+    }
+    const float ry = POST ? p.rstd[t] : 1.f, rh = NEXT ? p.rstd[p.T + t] : 0.f;
+    const float2 alpha2 = both(p.alpha), rh2 = both(rh), yg2 = both(ry * gt);
+    float2 h[NV][N2], e[NV][N2];
+    float2 s0 = both(0.f), s1 = both(0.f), s2 = both(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + i * tpr < chunks) {
+        const uint32_t src = at + (uint32_t)(i * tpr) * 16;
+        float2 v[N2], f[N2];
+        // v = w y (g): what the norm's sum takes the gradient times
+        unpack16(lds16(src), v, T());
+        if (POST) {
+          load_piece<T, P>(p.w, tid + i * tpr, f);
+#pragma unroll
+          for (int j = 0; j < N2; ++j) v[j] = mul2(v[j], f[j]);
+        }
+        if (GATE != 0) {
+          if (GATE == 1) load_gate_piece<T>(p, tid + i * tpr, f); else unpack16(lds16(src + at_g), f, T());
+#pragma unroll
+          for (int j = 0; j < N2; ++j) v[j] = mul2(v[j], f[j]);
+        }
+        if (res) {
+          unpack16(lds16(src + at_r), f, T());
+#pragma unroll
+          for (int j = 0; j < N2; ++j) h[i][j] = fma2(v[j], yg2, mul2(f[j], alpha2));
+        } else {
+#pragma unroll
+          for (int j = 0; j < N2; ++j) h[i][j] = mul2(v[j], yg2);
+        }
+        if (has_dh) {
+          unpack16(lds16(src + at_h), e[i], T());
+        } else {
+#pragma unroll
+          for (int j = 0; j < N2; ++j) e[i][j] = both(0.f);
+        }
+        if (has_dn) {
+          float2 d[N2];
+          unpack16(lds16(src + at_n), d, T());
+          load_piece<T, P>(p.wn, tid + i * tpr, f);
+#pragma unroll
+          for (int j = 0; j < N2; ++j) {
+            d[j] = mul2(d[j], f[j]);
+            e[i][j] = fma2(d[j], rh2, e[i][j]);
+            s0 = fma2(d[j], h[i][j], s0);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < N2; ++j) {
+          s1 = fma2(v[j], e[i][j], s1);
+          if (NEXT) s2 = fma2(v[j], h[i][j], s2);
+        }
+      }
+    float sum[3] = {s0.x + s0.y, s1.x + s1.y, s2.x + s2.y};
+    if (POST || NEXT || token) red.sum(sum);
+    const float c3 = NEXT ? rh * rh * rh * sum[0] * inv_h : 0.f;
+    const float raw = sum[1] - c3 * sum[2];
+    const float cy = POST ? ry * ry * ry * gt * raw * inv_h : 0.f;
+    if (token && tid == 0 && b.dgate != nullptr) {
+      const float one[1] = {ry * raw};
+      store_param<T, 1>(b.dgate, p.gate_f32, t, one);
+    }
+    const float2 c32 = both(-c3), cy2 = both(-cy), ry2 = both(ry);
+    uint4* dyo = reinterpret_cast<uint4*>(static_cast<T*>(b.dy) + t * p.H) + tid;
+    uint4* dro = reinterpret_cast<uint4*>(static_cast<T*>(b.dr) + t * p.H) + tid;
+    uint4* dgo = reinterpret_cast<uint4*>(static_cast<T*>(b.dgate) + t * p.H) + tid;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + i * tpr < chunks) {
+        const uint32_t src = at + (uint32_t)(i * tpr) * 16;
+        float2 y[N2], f[N2], d[N2];
+        if (has_dn) {
+          unpack16(lds16(src + at_n), f, T());
+#pragma unroll
+          for (int j = 0; j < N2; ++j) an[i][j] = fma2(f[j], mul2(h[i][j], rh2), an[i][j]);
+        }
+#pragma unroll
+        for (int j = 0; j < N2; ++j) d[j] = NEXT ? fma2(h[i][j], c32, e[i][j]) : e[i][j];
+        if (b.dr != nullptr) {
+#pragma unroll
+          for (int j = 0; j < N2; ++j) f[j] = mul2(d[j], alpha2);
+          dro[i * tpr] = pack16(f, T());
+        }
+        unpack16(lds16(src), y, T());
+        if (GATE == 0) {
+#pragma unroll
+          for (int j = 0; j < N2; ++j) d[j] = mul2(d[j], both(gt));
+        }
+        if (POST) load_piece<T, P>(p.w, tid + i * tpr, f);
+        if (GATE != 0) {
+          float2 g[N2], dg[N2];
+          if (GATE == 1) load_gate_piece<T>(p, tid + i * tpr, g); else unpack16(lds16(src + at_g), g, T());
+#pragma unroll
+          for (int j = 0; j < N2; ++j) {
+            const float2 u = POST ? mul2(mul2(y[j], ry2), f[j]) : y[j];
+            if (GATE == 1) ag[i][j] = fma2(d[j], u, ag[i][j]); else dg[j] = mul2(d[j], u);
+            d[j] = mul2(d[j], g[j]);
+          }
+          if (GATE == 2 && b.dgate != nullptr) dgo[i * tpr] = pack16(dg, T());
+        }
+        // d is the gradient of u now
+        if (POST) {
+#pragma unroll
+          for (int j = 0; j < N2; ++j) {
+            aw[i][j] = fma2(d[j], mul2(y[j], ry2), aw[i][j]);
+            d[j] = fma2(d[j], mul2(f[j], ry2), mul2(y[j], cy2));
+          }
+        }
+        if (b.dy != nullptr) dyo[i * tpr] = pack16(d, T());
+      }
+    const uint32_t swap = at;
+    at = other;
+    other = swap;
+  }
+  if (b.part != nullptr) {
+    float2* o = reinterpret_cast<float2*>(b.part + (int64_t)blockIdx.x * 3 * p.H);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = tid + i * tpr;
+      if (c < chunks) {
+#pragma unroll
+        for (int j = 0; j < N2; ++j) {
+          if (POST && b.want_dw) o[c * N2 + j] = aw[i][j];
+          if (NEXT && b.want_dwn) o[p.H / 2 + c * N2 + j] = an[i][j];
+          if (GATE == 1 && b.want_dgc) o[p.H + c * N2 + j] = ag[i][j];
+        }
+      }
+    }
+  }
+}
+
 // dst[c] = sum over the partial rows, in ascending order within eight interleaved groups that are then added in order.
 struct ColumnSumParams {
   const float* part;
@@ -314,10 +691,60 @@ bool vector_ok(const NormParams& p) {
          (p.gate_kind == B200MOE_GATE_TOKEN || aligned16(p.gate)) && aligned16(p.wn) && aligned16(p.h) && aligned16(p.n) && aligned16(p.q);
 }
 
+// The ring needs its gate rows in the rows' type, its weights in one type, a width that gives whole warps something to do,
+// and more rows than the SMs take at once.
+template <typename T>
+bool ring_ok(const NormParams& p, bool vec) {
+  return vec && p.H >= 512 && p.T >= 4 * device_sm_count() && (sizeof(T) == 4 || p.w == nullptr || p.wn == nullptr || p.w_f32 == p.wn_f32) &&
+         (p.gate_kind != B200MOE_GATE_FULL || sizeof(T) == 4 || !p.gate_f32);
+}
+// whether the weights are fp32 (they are of one type)
+bool fp32_weights(const NormParams& p) { return (p.w != nullptr && p.w_f32) || (p.wn != nullptr && p.wn_f32); }
+int ring_gate(const NormParams& p) {
+  return p.gate_kind == B200MOE_GATE_CHANNEL ? 1 : p.gate_kind == B200MOE_GATE_FULL ? 2 : 0;
+}
+template <typename T, typename P, bool POST, bool HOLD>
+void (*fwd_ring_g(int g))(NormParams) {
+  return g == 0 ? block_norm_ring_kernel<T, P, POST, 0, HOLD> : g == 1 ? block_norm_ring_kernel<T, P, POST, 1, HOLD>
+                                                                      : block_norm_ring_kernel<T, P, POST, 2, HOLD>;
+}
+template <typename T, typename P>
+void (*fwd_ring(const NormParams& p, bool hold))(NormParams) {
+  const int g = ring_gate(p);
+  if (p.w != nullptr) return hold ? fwd_ring_g<T, P, true, true>(g) : fwd_ring_g<T, P, true, false>(g);
+  return hold ? fwd_ring_g<T, P, false, true>(g) : fwd_ring_g<T, P, false, false>(g);
+}
+template <typename T, typename P, int GATE>
+void (*bwd_ring_g(const NormParams& p))(NormBwdParams) {
+  if (p.w != nullptr)
+    return p.wn != nullptr ? block_norm_bwd_ring_kernel<T, P, GATE, true, true> : block_norm_bwd_ring_kernel<T, P, GATE, true, false>;
+  return p.wn != nullptr ? block_norm_bwd_ring_kernel<T, P, GATE, false, true> : block_norm_bwd_ring_kernel<T, P, GATE, false, false>;
+}
+template <typename T, typename P>
+void (*bwd_ring(const NormParams& p))(NormBwdParams) {
+  const int g = ring_gate(p);
+  return g == 0 ? bwd_ring_g<T, P, 0>(p) : g == 1 ? bwd_ring_g<T, P, 1>(p) : bwd_ring_g<T, P, 2>(p);
+}
+
 template <typename T>
 int launch_norm_t(const NormParams& p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = vector_ok<T>(p);
+  if (ring_ok<T>(p, vec)) {
+    constexpr int NV = kNormValues / V;
+    const int tpr = (int)round_up64((p.H / V + NV - 1) / NV, 32);
+    const int arrays = 1 + (p.r != nullptr) + (p.gate_kind == B200MOE_GATE_FULL);
+    const int smem = 2 * arrays * p.H * (int)sizeof(T);
+    if (smem <= kRingLimit && tpr <= kNoHoldThreads) {
+      const bool hold = 2 * tpr <= kHoldThreads;
+      const int per_sm = std::max(1, std::min((hold ? kHoldThreads : kNoHoldThreads) / tpr, kRingLimit / (smem + 2048)));
+      const int grid = (int)std::min<int64_t>(p.T, (int64_t)device_sm_count() * per_sm);
+      void (*k)(NormParams) = fp32_weights(p) ? fwd_ring<T, float>(p, hold) : fwd_ring<T, T>(p, hold);
+      B200_CHECK_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingLimit));
+      B200_CHECK_CUDA(launch_chained(k, dim3(grid), dim3(tpr), smem, st, p));
+      return 0;
+    }
+  }
   const RowShape s = row_shape(vec ? p.H / V : p.H);
   const dim3 block(s.tpr, s.rows);
   const int per_sm = std::max(1, ((V * s.nv <= 8) ? 1024 : 512) / (s.tpr * s.rows));
@@ -353,14 +780,26 @@ int launch_norm_bwd_t(const NormBwdParams& b, const ColumnSumParams& sums, cudaS
   const NormParams& p = b.f;
   const bool vec = vector_ok<T>(p) && aligned16(b.dh) && aligned16(b.dn) && aligned16(b.dy) && aligned16(b.dr) &&
                    (p.gate_kind == B200MOE_GATE_TOKEN || aligned16(b.dgate));
-  const BwdShape r = bwd_shape<T>(p, vec);
+  BwdShape r = bwd_shape<T>(p, vec);
+  constexpr int NV = 16 / V;
+  const int arrays = 1 + (p.r != nullptr) + (b.dh != nullptr) + (b.dn != nullptr) + (p.gate_kind == B200MOE_GATE_FULL);
+  const int row_bytes = arrays * p.H * (int)sizeof(T);
+  const int tpr = (int)round_up64((p.H / V + NV - 1) / NV, 32);
+  const bool ring = ring_ok<T>(p, vec) && tpr <= kRowThreads && 2 * row_bytes <= kRingLimit;
   void (*k)(NormBwdParams) = nullptr;
-  if (vec)
+  if (ring) {
+    const int per_sm = std::max(1, std::min(kRowThreads / tpr, kRingLimit / (2 * row_bytes + 2048)));
+    r.grid = (int)std::min<int64_t>(p.T, (int64_t)device_sm_count() * per_sm);
+    r.s.rows = 1;
+    void (*kr)(NormBwdParams) = fp32_weights(p) ? bwd_ring<T, float>(p) : bwd_ring<T, T>(p);
+    B200_CHECK_CUDA(cudaFuncSetAttribute(kr, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingLimit));
+    B200_CHECK_CUDA(launch_chained(kr, dim3(r.grid), dim3(tpr), 2 * (size_t)row_bytes, st, b));
+  } else if (vec)
     k = r.s.nv == 1 ? block_norm_bwd_kernel<T, V, 1> : r.s.nv == 2 ? block_norm_bwd_kernel<T, V, 2>
         : r.s.nv == 4 ? block_norm_bwd_kernel<T, V, 4> : block_norm_bwd_kernel<T, V, kMaxPieces<T>>;
   else
     k = r.s.nv <= 2 ? block_norm_bwd_kernel<T, 1, 2> : r.s.nv <= 8 ? block_norm_bwd_kernel<T, 1, 8> : block_norm_bwd_kernel<T, 1, 32>;
-  B200_CHECK_CUDA(launch_chained(k, dim3(r.grid), dim3(r.s.tpr, r.s.rows), 0, st, b));
+  if (!ring) B200_CHECK_CUDA(launch_chained(k, dim3(r.grid), dim3(r.s.tpr, r.s.rows), 0, st, b));
   if (b.part != nullptr) {
     ColumnSumParams c = sums;
     c.part = b.part;
@@ -384,8 +823,9 @@ static int check_norm(int64_t y_stride, int64_t r_stride, int64_t gate_stride, i
 }
 
 int64_t block_norm_bwd_workspace(int T, int H, int dtype) {
-  // rows of partial sums: the larger of the two shapes that a call of this size can take
-  int64_t rows = 0;
+  // rows of partial sums: the largest of the shapes that a call of this size can take (the ring's CTAs hold 16 values a thread)
+  const int ring_per_sm = std::max(1, kRowThreads / (int)round_up64((H + 15) / 16, 32));
+  int64_t rows = std::min<int64_t>(T, (int64_t)device_sm_count() * ring_per_sm);
   for (int vec = 0; vec < 2; ++vec) {
     const RowShape s = row_shape(vec ? (H + (dtype == B200MOE_T_FP32 ? 3 : 7)) / (dtype == B200MOE_T_FP32 ? 4 : 8) : H);
     rows = std::max(rows, std::min<int64_t>((T + s.rows - 1) / s.rows, device_sm_count()) * s.rows);

@@ -56,14 +56,14 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 template <int LPR>
 __device__ __forceinline__ uint32_t group_max(uint32_t v) {
-  if (LPR == 32) return __reduce_max_sync(0xffffffffu, v);
+  if constexpr (LPR == 32) return __reduce_max_sync(0xffffffffu, v);
 #pragma unroll
   for (int d = LPR / 2; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;
 }
 template <int LPR>
 __device__ __forceinline__ uint32_t group_min(uint32_t v) {
-  if (LPR == 32) return __reduce_min_sync(0xffffffffu, v);
+  if constexpr (LPR == 32) return __reduce_min_sync(0xffffffffu, v);
 #pragma unroll
   for (int d = LPR / 2; d > 0; d >>= 1) v = min(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;

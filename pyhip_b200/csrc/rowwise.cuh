@@ -66,6 +66,87 @@ __device__ __forceinline__ void store_param(void* p, bool f32, int64_t at, const
   }
 }
 
+// 16 bytes, global to shared, asynchronously; groups complete in order, and a thread that reads only what it copied itself
+// needs no barrier
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+
+// Two fp32 values to an instruction (fma.rn.f32x2): the row kernels are close to the issue rate, not to the FMA rate.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// 16 bytes of a row's type <-> pairs of fp32
+template <typename T> constexpr int kPairs = 8 / (int)sizeof(T);
+__device__ __forceinline__ void unpack16(const uint4& v, float2 (&o)[2], float) {
+  o[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+  o[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+}
+__device__ __forceinline__ void unpack16(const uint4& v, float2 (&o)[4], __nv_bfloat16) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void unpack16(const uint4& v, float2 (&o)[4], __half) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+}
+__device__ __forceinline__ uint4 pack16(const float2 (&v)[2], float) {
+  return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+}
+__device__ __forceinline__ uint4 pack16(const float2 (&v)[4], __nv_bfloat16) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 k = __float22bfloat162_rn(v[i]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&k);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 pack16(const float2 (&v)[4], __half) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 k = __float22half2_rn(v[i]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&k);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// the parameters of piece c of a row of T, held as T or as fp32
+template <typename T, typename P, int N2>
+__device__ __forceinline__ void load_piece(const void* p, int c, float2 (&o)[N2]) {
+  static_assert(N2 == kPairs<T>, "a piece of the row's type");
+  if constexpr (sizeof(P) == sizeof(T)) {
+    unpack16(static_cast<const uint4*>(p)[c], o, T());
+  } else {
+    const float4 a = static_cast<const float4*>(p)[2 * c], b = static_cast<const float4*>(p)[2 * c + 1];
+    o[0] = make_float2(a.x, a.y); o[1] = make_float2(a.z, a.w);
+    o[2] = make_float2(b.x, b.y); o[3] = make_float2(b.z, b.w);
+  }
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -110,6 +191,61 @@ struct RowReduce {
     __syncthreads();
     const int lane = threadIdx.x & 31;
     return __reduce_max_sync(0xffffffffu, lane < wpr ? s[w0 + lane] : 0u);
+  }
+};
+
+// The same for CTAs whose threads all share the row, or N rows that are reduced together: after the barrier every thread
+// reads the warps' sums four at a time instead of going through the tree again.
+struct CtaReduce {
+  float* slots;   // [2][3][32], 16-byte aligned
+  uint32_t turn;
+  __device__ explicit CtaReduce(float* s) : slots(s), turn(0) {
+    for (int i = threadIdx.x; i < 2 * 3 * 32; i += blockDim.x) s[i] = 0.f;
+    __syncthreads();
+  }
+  template <int N>
+  __device__ __forceinline__ void sum(float (&v)[N]) {
+    static_assert(N <= 3, "three sums at most");
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+    float* s = slots + turn * 3 * 32;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i * 32 + (threadIdx.x >> 5)] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float4* q = reinterpret_cast<const float4*>(s + i * 32);
+      float4 a = q[0];
+      for (int k = 1; k < ((int)blockDim.x + 127) / 128; ++k) {
+        const float4 b = q[k];
+        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+      }
+      v[i] = (a.x + a.y) + (a.z + a.w);
+    }
+  }
+  template <int N>
+  __device__ __forceinline__ void max_u32(uint32_t (&v)[N]) {
+    static_assert(N <= 3, "three values at most");
+    uint32_t* s = reinterpret_cast<uint32_t*>(slots + turn * 3 * 32);
+    turn ^= 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = __reduce_max_sync(0xffffffffu, v[i]);
+      if ((threadIdx.x & 31) == 0) s[i * 32 + (threadIdx.x >> 5)] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint4* q = reinterpret_cast<const uint4*>(s + i * 32);
+      v[i] = 0;
+      for (int k = 0; k < ((int)blockDim.x + 127) / 128; ++k) {
+        const uint4 b = q[k];
+        v[i] = max(v[i], max(max(b.x, b.y), max(b.z, b.w)));
+      }
+    }
   }
 };
 

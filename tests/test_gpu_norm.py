@@ -38,7 +38,8 @@ def _inputs(T, H, dtype, pdtype, post, gate, nxt, residual=True, seed=0):
     return i
 
 
-WIDTHS = [(1, 1), (3, 7), (2, 32), (70, 64), (33, 288), (5, 1001), (40, 2880), (3, 4104), (9, 7168), (2, 8193), (2, 16384), (1, 16383)]
+WIDTHS = [(1, 1), (3, 7), (2, 32), (70, 64), (33, 288), (5, 1001), (40, 2880), (3, 4104), (9, 7168), (2, 8193), (2, 16384), (1, 16383),
+          (700, 2880), (593, 520), (600, 1000), (1300, 7168), (595, 16384)]        # the last ones take the ring where it applies
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
@@ -72,7 +73,8 @@ def _grads(i, r, dh, dn):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("T,H", [(1, 1), (3, 7), (70, 64), (300, 288), (5, 1001), (700, 2880), (3, 4104), (160, 7168), (2, 8193), (2, 16384), (1, 16383)])
+@pytest.mark.parametrize("T,H", [(1, 1), (3, 7), (70, 64), (300, 288), (5, 1001), (700, 2880), (3, 4104), (160, 7168), (2, 8193), (2, 16384), (1, 16383),
+                                 (593, 520), (1300, 1000), (620, 8192), (595, 16384)])
 def test_backward_matches_64_bits(T, H, dtype):
     for k, (post, gate, nxt, pdtype) in enumerate([(True, "channel", True, torch.float32), (True, None, False, dtype), (False, "token", True, dtype),
                                                    (True, "token", True, dtype), (True, "full", True, dtype), (False, "full", False, torch.float32),
