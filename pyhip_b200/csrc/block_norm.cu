@@ -150,7 +150,7 @@ block_norm_kernel(const __grid_constant__ NormParams p) {
 
 // piece c of a gate per channel, which is fp32 or of the rows' type whatever the weights are
 template <typename T, int N2>
-__device__ __forceinline__ void load_gate_piece(const NormParams& p, int c, float2 (&o)[N2]) {
+__device__ __forceinline__ void load_gate_piece(const NormParams& p, int c, f32x2 (&o)[N2]) {
   if (p.gate_f32) load_piece<T, float>(p.gate, c, o); else load_piece<T, T>(p.gate, c, o);
 }
 
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(HOLD ? kHoldThreads : kNoHoldThreads, 1)
 block_norm_ring_kernel(const __grid_constant__ NormParams p) {
   constexpr int VEC = 16 / sizeof(T), NV = kNormValues / VEC, N2 = VEC / 2;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ __align__(16) float slots[2 * 3 * 32];
+  __shared__ __align__(16) float slots[2 * 32 * 4];
   CtaReduce red(slots);
   grid_dep_wait();
   grid_dep_launch();
@@ -195,12 +195,12 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
     copy_commit();
   };
   // the factor of y in piece c that the rows share, and the next norm's weights
-  auto load_factor = [&](int c, float2 (&f)[N2]) {
+  auto load_factor = [&](int c, f32x2 (&f)[N2]) {
 #pragma unroll
     for (int j = 0; j < N2; ++j) f[j] = both(1.f);
     if (POST) load_piece<T, P>(p.w, c, f);
     if (GATE == 1) {
-      float2 g[N2];
+      f32x2 g[N2];
       load_gate_piece<T>(p, c, g);
 #pragma unroll
       for (int j = 0; j < N2; ++j) f[j] = mul2(f[j], g[j]);
@@ -208,7 +208,7 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
   };
   const int64_t step = gridDim.x;
   fetch(blockIdx.x, mine);
-  float2 hold_f[HOLD ? NV : 1][N2], hold_n[HOLD ? NV : 1][N2];
+  f32x2 hold_f[HOLD ? NV : 1][N2], hold_n[HOLD ? NV : 1][N2];
   if (HOLD) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -221,10 +221,10 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
   for (int64_t t = blockIdx.x; t < p.T; t += step) {
     copy_wait<0>();
     fetch(t + step, other);                       // the stage that the row before has left
-    float2 h[NV][N2];
+    f32x2 h[NV][N2];
     float scale = 1.f;                            // rstd(y) and a token's gate
     if (POST) {
-      float2 ss = both(0.f);
+      f32x2 ss = both(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (tid + i * tpr < chunks) {
@@ -232,9 +232,8 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
 #pragma unroll
           for (int j = 0; j < N2; ++j) ss = fma2(h[i][j], h[i][j], ss);
         }
-      float sum[1] = {ss.x + ss.y};
-      red.sum(sum);
-      scale = rsqrtf(sum[0] * inv_h + p.eps);
+      const float sum = red.sum(both_of(ss));
+      scale = rsqrtf(sum * inv_h + p.eps);
       if (tid == 0 && p.rstd != nullptr) p.rstd[t] = scale;
     }
     if (GATE == 0 && p.gate_kind == B200MOE_GATE_TOKEN) {
@@ -242,14 +241,14 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
       load_param<T, 1>(p.gate, p.gate_f32, t * p.gate_stride, g1);
       scale *= g1[0];
     }
-    const float2 scale2 = both(scale), alpha2 = both(p.alpha);
-    float2 ss = both(0.f);
+    const f32x2 scale2 = both(scale), alpha2 = both(p.alpha);
+    f32x2 ss = both(0.f);
     uint4* ho = reinterpret_cast<uint4*>(static_cast<T*>(p.h) + t * p.H) + tid;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (tid + i * tpr < chunks) {
         const uint32_t src = at + (uint32_t)(i * tpr) * 16;
-        float2 f[N2], r[N2];
+        f32x2 f[N2], r[N2];
         if (!POST) unpack16(lds16(src), h[i], T());
         if (HOLD) {
 #pragma unroll
@@ -274,16 +273,15 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
         if (p.h != nullptr) ho[i * tpr] = pack16(h[i], T());
       }
     if (next) {
-      float sum[1] = {ss.x + ss.y};
-      red.sum(sum);
-      const float rh = rsqrtf(sum[0] * inv_h + p.eps);
+      const float sum = red.sum(both_of(ss));
+      const float rh = rsqrtf(sum * inv_h + p.eps);
       if (tid == 0 && p.rstd != nullptr) p.rstd[p.T + t] = rh;
-      const float2 rh2 = both(rh);
+      const f32x2 rh2 = both(rh);
       uint4* no = reinterpret_cast<uint4*>(static_cast<T*>(p.n) + t * p.H) + tid;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (tid + i * tpr < chunks) {
-          float2 f[N2];
+          f32x2 f[N2];
           if (HOLD) {
 #pragma unroll
             for (int j = 0; j < N2; ++j) f[j] = hold_n[i][j];
@@ -296,17 +294,19 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
         }
     }
     if (p.q != nullptr) {
-      uint32_t m[1] = {0};
+      uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (tid + i * tpr < chunks) {
 #pragma unroll
-          for (int j = 0; j < N2; ++j)
-            m[0] = max(m[0], max(__float_as_uint(h[i][j].x) & 0x7fffffffu, __float_as_uint(h[i][j].y) & 0x7fffffffu));
+          for (int j = 0; j < N2; ++j) {
+            const float2 v = split(h[i][j]);
+            m = max(m, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
+          }
         }
-      red.max_u32(m);
-      const float sc = int8_scale(m[0]);
-      const bool bad = m[0] >= 0x7f800000u;
+      m = red.max_u32(m);
+      const float sc = int8_scale(m);
+      const bool bad = m >= 0x7f800000u;
       const float inv = __frcp_rn(sc);
       if (tid == 0) p.q_scale[t] = sc;
 #pragma unroll
@@ -316,8 +316,9 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
           Pack<int8_t, VEC> k;
 #pragma unroll
           for (int j = 0; j < N2; ++j) {
-            k.v[2 * j] = bad ? (int8_t)0 : (int8_t)quant_int8(h[i][j].x, sc, inv);
-            k.v[2 * j + 1] = bad ? (int8_t)0 : (int8_t)quant_int8(h[i][j].y, sc, inv);
+            const float2 v = split(h[i][j]);
+            k.v[2 * j] = bad ? (int8_t)0 : (int8_t)quant_int8(v.x, sc, inv);
+            k.v[2 * j + 1] = bad ? (int8_t)0 : (int8_t)quant_int8(v.y, sc, inv);
           }
           *reinterpret_cast<Pack<int8_t, VEC>*>(p.q + t * p.H + c * VEC) = k;
         }
@@ -454,7 +455,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
   constexpr int VEC = 16 / sizeof(T), NV = 16 / VEC, N2 = VEC / 2;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ __align__(16) float slots[2 * 3 * 32];
+  __shared__ __align__(16) float slots[2 * 32 * 4];
   const NormParams& p = b.f;
   CtaReduce red(slots);
   grid_dep_wait();
@@ -488,7 +489,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
     }
     copy_commit();
   };
-  float2 aw[POST ? NV : 1][N2], an[NEXT ? NV : 1][N2], ag[GATE == 1 ? NV : 1][N2];
+  f32x2 aw[POST ? NV : 1][N2], an[NEXT ? NV : 1][N2], ag[GATE == 1 ? NV : 1][N2];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -510,14 +511,14 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
       gt = g1[0];
     }
     const float ry = POST ? p.rstd[t] : 1.f, rh = NEXT ? p.rstd[p.T + t] : 0.f;
-    const float2 alpha2 = both(p.alpha), rh2 = both(rh), yg2 = both(ry * gt);
-    float2 h[NV][N2], e[NV][N2];
-    float2 s0 = both(0.f), s1 = both(0.f), s2 = both(0.f);
+    const f32x2 alpha2 = both(p.alpha), rh2 = both(rh), yg2 = both(ry * gt);
+    f32x2 h[NV][N2], e[NV][N2];
+    f32x2 s0 = both(0.f), s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (tid + i * tpr < chunks) {
         const uint32_t src = at + (uint32_t)(i * tpr) * 16;
-        float2 v[N2], f[N2];
+        f32x2 v[N2], f[N2];
         // v = w y (g): what the norm's sum takes the gradient times
         unpack16(lds16(src), v, T());
         if (POST) {
@@ -545,7 +546,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
           for (int j = 0; j < N2; ++j) e[i][j] = both(0.f);
         }
         if (has_dn) {
-          float2 d[N2];
+          f32x2 d[N2];
           unpack16(lds16(src + at_n), d, T());
           load_piece<T, P>(p.wn, tid + i * tpr, f);
 #pragma unroll
@@ -561,16 +562,16 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
           if (NEXT) s2 = fma2(v[j], h[i][j], s2);
         }
       }
-    float sum[3] = {s0.x + s0.y, s1.x + s1.y, s2.x + s2.y};
-    if (POST || NEXT || token) red.sum(sum);
-    const float c3 = NEXT ? rh * rh * rh * sum[0] * inv_h : 0.f;
-    const float raw = sum[1] - c3 * sum[2];
+    float t0 = both_of(s0), t1 = both_of(s1), t2 = both_of(s2);
+    if (POST || NEXT || token) red.sum3(t0, t1, t2);
+    const float c3 = NEXT ? rh * rh * rh * t0 * inv_h : 0.f;
+    const float raw = t1 - c3 * t2;
     const float cy = POST ? ry * ry * ry * gt * raw * inv_h : 0.f;
     if (token && tid == 0 && b.dgate != nullptr) {
       const float one[1] = {ry * raw};
       store_param<T, 1>(b.dgate, p.gate_f32, t, one);
     }
-    const float2 c32 = both(-c3), cy2 = both(-cy), ry2 = both(ry);
+    const f32x2 c32 = both(-c3), cy2 = both(-cy), ry2 = both(ry);
     uint4* dyo = reinterpret_cast<uint4*>(static_cast<T*>(b.dy) + t * p.H) + tid;
     uint4* dro = reinterpret_cast<uint4*>(static_cast<T*>(b.dr) + t * p.H) + tid;
     uint4* dgo = reinterpret_cast<uint4*>(static_cast<T*>(b.dgate) + t * p.H) + tid;
@@ -578,7 +579,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
     for (int i = 0; i < NV; ++i)
       if (tid + i * tpr < chunks) {
         const uint32_t src = at + (uint32_t)(i * tpr) * 16;
-        float2 y[N2], f[N2], d[N2];
+        f32x2 y[N2], f[N2], d[N2];
         if (has_dn) {
           unpack16(lds16(src + at_n), f, T());
 #pragma unroll
@@ -598,11 +599,11 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
         }
         if (POST) load_piece<T, P>(p.w, tid + i * tpr, f);
         if (GATE != 0) {
-          float2 g[N2], dg[N2];
+          f32x2 g[N2], dg[N2];
           if (GATE == 1) load_gate_piece<T>(p, tid + i * tpr, g); else unpack16(lds16(src + at_g), g, T());
 #pragma unroll
           for (int j = 0; j < N2; ++j) {
-            const float2 u = POST ? mul2(mul2(y[j], ry2), f[j]) : y[j];
+            const f32x2 u = POST ? mul2(mul2(y[j], ry2), f[j]) : y[j];
             if (GATE == 1) ag[i][j] = fma2(d[j], u, ag[i][j]); else dg[j] = mul2(d[j], u);
             d[j] = mul2(d[j], g[j]);
           }
@@ -623,7 +624,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
     other = swap;
   }
   if (b.part != nullptr) {
-    float2* o = reinterpret_cast<float2*>(b.part + (int64_t)blockIdx.x * 3 * p.H);
+    f32x2* o = reinterpret_cast<f32x2*>(b.part + (int64_t)blockIdx.x * 3 * p.H);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = tid + i * tpr;

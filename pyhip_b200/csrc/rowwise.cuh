@@ -80,70 +80,86 @@ __device__ __forceinline__ uint4 lds16(uint32_t at) {
   return v;
 }
 
-// Two fp32 values to an instruction (fma.rn.f32x2): the row kernels are close to the issue rate, not to the FMA rate.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+// Two fp32 values to an instruction (fma.rn.f32x2): the row kernels are close to the issue rate, not to the FMA rate.  A pair
+// is one 64-bit value, so that it stays in a pair of neighbouring registers.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
   return d;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+__device__ __forceinline__ float2 split(f32x2 v) {
   float2 d;
-  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
   return d;
 }
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float both_of(f32x2 v) {
+  const float2 d = split(v);
+  return d.x + d.y;
+}
+__device__ __forceinline__ f32x2 both(float v) { return pair(v, v); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 
 // 16 bytes of a row's type <-> pairs of fp32
 template <typename T> constexpr int kPairs = 8 / (int)sizeof(T);
-__device__ __forceinline__ void unpack16(const uint4& v, float2 (&o)[2], float) {
-  o[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
-  o[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+__device__ __forceinline__ void unpack16(const uint4& v, f32x2 (&o)[2], float) {
+  o[0] = pair(__uint_as_float(v.x), __uint_as_float(v.y));
+  o[1] = pair(__uint_as_float(v.z), __uint_as_float(v.w));
 }
-__device__ __forceinline__ void unpack16(const uint4& v, float2 (&o)[4], __nv_bfloat16) {
+__device__ __forceinline__ void unpack16(const uint4& v, f32x2 (&o)[4], __nv_bfloat16) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  for (int i = 0; i < 4; ++i) o[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
-__device__ __forceinline__ void unpack16(const uint4& v, float2 (&o)[4], __half) {
+__device__ __forceinline__ void unpack16(const uint4& v, f32x2 (&o)[4], __half) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    o[i] = pair(f.x, f.y);
+  }
 }
-__device__ __forceinline__ uint4 pack16(const float2 (&v)[2], float) {
-  return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+__device__ __forceinline__ uint4 pack16(const f32x2 (&v)[2], float) {
+  const float2 a = split(v[0]), b = split(v[1]);
+  return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
 }
-__device__ __forceinline__ uint4 pack16(const float2 (&v)[4], __nv_bfloat16) {
+__device__ __forceinline__ uint4 pack16(const f32x2 (&v)[4], __nv_bfloat16) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 k = __float22bfloat162_rn(v[i]);
+    const __nv_bfloat162 k = __float22bfloat162_rn(split(v[i]));
     w[i] = *reinterpret_cast<const uint32_t*>(&k);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ uint4 pack16(const float2 (&v)[4], __half) {
+__device__ __forceinline__ uint4 pack16(const f32x2 (&v)[4], __half) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 k = __float22half2_rn(v[i]);
+    const __half2 k = __float22half2_rn(split(v[i]));
     w[i] = *reinterpret_cast<const uint32_t*>(&k);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 // the parameters of piece c of a row of T, held as T or as fp32
 template <typename T, typename P, int N2>
-__device__ __forceinline__ void load_piece(const void* p, int c, float2 (&o)[N2]) {
+__device__ __forceinline__ void load_piece(const void* p, int c, f32x2 (&o)[N2]) {
   static_assert(N2 == kPairs<T>, "a piece of the row's type");
   if constexpr (sizeof(P) == sizeof(T)) {
     unpack16(static_cast<const uint4*>(p)[c], o, T());
   } else {
     const float4 a = static_cast<const float4*>(p)[2 * c], b = static_cast<const float4*>(p)[2 * c + 1];
-    o[0] = make_float2(a.x, a.y); o[1] = make_float2(a.z, a.w);
-    o[2] = make_float2(b.x, b.y); o[3] = make_float2(b.z, b.w);
+    o[0] = pair(a.x, a.y); o[1] = pair(a.z, a.w);
+    o[2] = pair(b.x, b.y); o[3] = pair(b.z, b.w);
   }
 }
 
@@ -194,58 +210,71 @@ struct RowReduce {
   }
 };
 
-// The same for CTAs whose threads all share the row, or N rows that are reduced together: after the barrier every thread
-// reads the warps' sums four at a time instead of going through the tree again.
+// Sums of four values over a warp with six exchanges: two lanes swap what the other keeps, so the values thin out while
+// the lanes are joined.  Lane l ends with the sum of value l & 3.
+__device__ __forceinline__ float warp_sum4(float a, float b, float c, float d) {
+  const int lane = threadIdx.x & 31;
+  const bool o1 = lane & 1, o2 = lane & 2;
+  float x = o1 ? b : a, y = o1 ? d : c;
+  x += __shfl_xor_sync(0xffffffffu, o1 ? a : b, 1);
+  y += __shfl_xor_sync(0xffffffffu, o1 ? c : d, 1);
+  float v = o2 ? y : x;
+  v += __shfl_xor_sync(0xffffffffu, o2 ? x : y, 2);
+#pragma unroll
+  for (int k = 4; k < 32; k <<= 1) v += __shfl_xor_sync(0xffffffffu, v, k);
+  return v;
+}
+
+// The same for CTAs whose threads all share the row.
 struct CtaReduce {
-  float* slots;   // [2][3][32], 16-byte aligned
+  float* slots;   // [2][32][4], 16-byte aligned; the entries of warps that do not exist stay zero
   uint32_t turn;
   __device__ explicit CtaReduce(float* s) : slots(s), turn(0) {
-    for (int i = threadIdx.x; i < 2 * 3 * 32; i += blockDim.x) s[i] = 0.f;
+    for (int i = threadIdx.x; i < 2 * 32 * 4; i += blockDim.x) s[i] = 0.f;
     __syncthreads();
   }
-  template <int N>
-  __device__ __forceinline__ void sum(float (&v)[N]) {
-    static_assert(N <= 3, "three sums at most");
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-    float* s = slots + turn * 3 * 32;
+  __device__ __forceinline__ float sum(float v) {
+    v = warp_sum(v);
+    float* s = slots + turn * 128;
     turn ^= 1;
-    if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) s[i * 32 + (threadIdx.x >> 5)] = v[i];
-    }
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float4* q = reinterpret_cast<const float4*>(s + i * 32);
-      float4 a = q[0];
-      for (int k = 1; k < ((int)blockDim.x + 127) / 128; ++k) {
-        const float4 b = q[k];
-        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-      }
-      v[i] = (a.x + a.y) + (a.z + a.w);
+    // the warps' sums, four at a time
+    const float4* q = reinterpret_cast<const float4*>(s);
+    float4 a = q[0];
+    for (int k = 1; k < ((int)blockDim.x + 127) / 128; ++k) {
+      const float4 b = q[k];
+      a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
     }
+    return (a.x + a.y) + (a.z + a.w);
   }
-  template <int N>
-  __device__ __forceinline__ void max_u32(uint32_t (&v)[N]) {
-    static_assert(N <= 3, "three values at most");
-    uint32_t* s = reinterpret_cast<uint32_t*>(slots + turn * 3 * 32);
+  // (the slots of a turn belong to one kind of reduction in a kernel: sum3 here, sum and max_u32 elsewhere)
+  __device__ __forceinline__ void sum3(float& a, float& b, float& c) {
+    const int lane = threadIdx.x & 31;
+    float v = warp_sum4(a, b, c, 0.f);
+    float* s = slots + turn * 128;
     turn ^= 1;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = __reduce_max_sync(0xffffffffu, v[i]);
-      if ((threadIdx.x & 31) == 0) s[i * 32 + (threadIdx.x >> 5)] = v[i];
-    }
+    if (lane < 4) s[(threadIdx.x >> 5) * 4 + lane] = v;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint4* q = reinterpret_cast<const uint4*>(s + i * 32);
-      v[i] = 0;
-      for (int k = 0; k < ((int)blockDim.x + 127) / 128; ++k) {
-        const uint4 b = q[k];
-        v[i] = max(v[i], max(max(b.x, b.y), max(b.z, b.w)));
-      }
+    const float4 q = reinterpret_cast<const float4*>(s)[lane];
+    v = warp_sum4(q.x, q.y, q.z, q.w);
+    a = __shfl_sync(0xffffffffu, v, 0);
+    b = __shfl_sync(0xffffffffu, v, 1);
+    c = __shfl_sync(0xffffffffu, v, 2);
+  }
+  __device__ __forceinline__ uint32_t max_u32(uint32_t v) {
+    uint32_t* s = reinterpret_cast<uint32_t*>(slots + turn * 128);
+    turn ^= 1;
+    v = __reduce_max_sync(0xffffffffu, v);
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const uint4* q = reinterpret_cast<const uint4*>(s);
+    v = 0;
+    for (int k = 0; k < ((int)blockDim.x + 127) / 128; ++k) {
+      const uint4 b = q[k];
+      v = max(v, max(max(b.x, b.y), max(b.z, b.w)));
     }
+    return v;
   }
 };
 
