@@ -19,41 +19,45 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _f32_bits(weight, gate, next_weight):
-    f = torch.float32
-    return ((weight is not None and weight.dtype == f) | (gate is not None and gate.dtype == f) << 1 |
-            (next_weight is not None and next_weight.dtype == f) << 2)
+_F32 = torch.float32
 
 
-def _gate_of(gate, kind):
-    """(tensor, elements between its rows) as the kernels read it."""
-    if gate is None:
-        return None, 0
-    if kind == _lib.GATE_FULL:
-        return rows_of(gate)
-    gate = gate.contiguous()
-    return gate, 1
+def _tensors(y, residual, weight, gate, kind, next_weight):
+    """What the C calls take first: addresses and row distances of the inputs, the size, the types, the gate's kind.  Second: the
+    tensors themselves, which may be copies and have to live until the launch."""
+    y2, ys = rows_of(y)
+    T, H = y2.shape
+    r2 = g2 = None
+    rs = gs = bits = 0
+    if residual is not None:
+        r2, rs = rows_of(residual)
+    if weight is not None:
+        weight = weight.contiguous()
+        bits = weight.dtype is _F32
+    if gate is not None:
+        g2, gs = rows_of(gate) if kind == _lib.GATE_FULL else (gate.contiguous(), 1)
+        bits |= (gate.dtype is _F32) << 1
+    if next_weight is not None:
+        next_weight = next_weight.contiguous()
+        bits |= (next_weight.dtype is _F32) << 2
+    return ((y2.data_ptr(), ys, None if r2 is None else r2.data_ptr(), rs, None if weight is None else weight.data_ptr(),
+             None if g2 is None else g2.data_ptr(), gs, None if next_weight is None else next_weight.data_ptr(), T, H,
+             ROW_TYPES[y.dtype], bits, kind), (y2, r2, weight, g2, next_weight))
 
 
 def _forward(y, residual, weight, gate, kind, next_weight, alpha, eps, want_h, quant, save):
-    dev, H = y.device, y.shape[-1]
-    y2, ys = rows_of(y)
-    T = y2.shape[0]
-    r2, rs = (None, 0) if residual is None else rows_of(residual)
-    g2, gs = _gate_of(gate, kind)
-    w = None if weight is None else weight.contiguous()
-    wn = None if next_weight is None else next_weight.contiguous()
-    h = torch.empty(y.shape, dtype=y.dtype, device=dev) if want_h else None
-    n = q = scale = None
+    args, _hold = _tensors(y, residual, weight, gate, kind, next_weight)
+    h = torch.empty(y.shape, dtype=y.dtype, device=y.device) if want_h else None
+    n = q = scale = rstd = None
     if quant:
-        q = torch.empty(y.shape, dtype=torch.int8, device=dev)
-        scale = torch.empty(y.shape[:-1], dtype=torch.float32, device=dev)
-    elif wn is not None:
-        n = torch.empty(y.shape, dtype=y.dtype, device=dev)
-    rstd = torch.empty(2, T, dtype=torch.float32, device=dev) if save else None
-    _lib.check(_lib.lib().b200moe_block_norm(
-        y2.data_ptr(), ys, _p(r2), rs, _p(w), _p(g2), gs, _p(wn), T, H, ROW_TYPES[y.dtype], _f32_bits(w, g2, wn), kind,
-        alpha, eps, _p(h), _p(n), _p(q), _p(scale), _p(rstd), stream_of(y)), "block_norm")
+        q = torch.empty(y.shape, dtype=torch.int8, device=y.device)
+        scale = torch.empty(y.shape[:-1], dtype=_F32, device=y.device)
+    elif next_weight is not None:
+        n = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    if save:
+        rstd = torch.empty(2 * args[8], dtype=_F32, device=y.device)
+    _lib.check(_lib.lib().b200moe_block_norm(*args, alpha, eps, _p(h), _p(n), _p(q), _p(scale), _p(rstd),
+                                             stream_of(y.get_device())), "block_norm")
     return h, n, q, scale, rstd
 
 
@@ -64,79 +68,86 @@ def _bwd_bytes(T, H, dt):
     return b.value
 
 
+def _backward(saved, need, how, dh, dn):
+    y, residual, weight, gate, next_weight, rstd = saved
+    kind, alpha = how
+    args, _hold = _tensors(y, residual, weight, gate, kind, next_weight)
+    if dh is not None:
+        dh = dh.contiguous()
+    if dn is not None:
+        dn = dn.contiguous()
+    dev = y.device
+    dy, dr, dw, dg, dwn = (torch.empty(t.shape, dtype=t.dtype, device=dev) if w else None
+                           for t, w in zip((y, residual, weight, gate, next_weight), need))
+    ws, size = None, 0
+    if dw is not None or dwn is not None or (dg is not None and kind == _lib.GATE_CHANNEL):
+        size = _bwd_bytes(args[8], args[9], args[10])
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _lib.check(_lib.lib().b200moe_block_norm_bwd(
+        *args, alpha, rstd.data_ptr(), _p(dh), _p(dn), _p(dy), _p(dr), _p(dw), _p(dg), _p(dwn), _p(ws), size,
+        stream_of(y.get_device())), "block_norm_bwd")
+    return dy, dr, dw, dg, dwn, None, None, None
+
+
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, residual, weight, gate, next_weight, kind, alpha, eps, want_h):
-        with on_device(y):
-            h, n, _, _, rstd = _forward(y, residual, weight, gate, kind, next_weight, alpha, eps, want_h, False, True)
+    def forward(ctx, y, residual, weight, gate, next_weight, how, eps, want_h):
+        h, n, _, _, rstd = on_device(y.get_device(), _forward, y, residual, weight, gate, how[0], next_weight, how[1], eps, want_h,
+                                     False, True)
         ctx.save_for_backward(y, residual, weight, gate, next_weight, rstd)
-        ctx.kind, ctx.alpha = kind, alpha
+        ctx.how = how
         ctx.set_materialize_grads(False)
         return h, n
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dn):
-        y, residual, weight, gate, next_weight, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        with on_device(y):
-            dev, H, dt = y.device, y.shape[-1], ROW_TYPES[y.dtype]
-            y2, ys = rows_of(y)
-            T = y2.shape[0]
-            r2, rs = (None, 0) if residual is None else rows_of(residual)
-            g2, gs = _gate_of(gate, ctx.kind)
-            w = None if weight is None else weight.contiguous()
-            wn = None if next_weight is None else next_weight.contiguous()
-            dh = None if dh is None else dh.contiguous()
-            dn = None if dn is None else dn.contiguous()
-
-            def like(t, wanted):
-                return torch.empty(t.shape, dtype=t.dtype, device=dev) if wanted else None
-
-            dy, dr = like(y, need[0]), like(residual, need[1])
-            dw, dg, dwn = like(weight, need[2]), like(gate, need[3]), like(next_weight, need[4])
-            ws, size = None, 0
-            if dw is not None or dwn is not None or (dg is not None and ctx.kind == _lib.GATE_CHANNEL):
-                size = _bwd_bytes(T, H, dt)
-                ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            _lib.check(_lib.lib().b200moe_block_norm_bwd(
-                y2.data_ptr(), ys, _p(r2), rs, _p(w), _p(g2), gs, _p(wn), T, H, dt, _f32_bits(w, g2, wn), ctx.kind, ctx.alpha,
-                rstd.data_ptr(), _p(dh), _p(dn), _p(dy), _p(dr), _p(dw), _p(dg), _p(dwn), _p(ws), size, stream_of(y)),
-                "block_norm_bwd")
-        return dy, dr, dw, dg, dwn, None, None, None, None
+        saved = ctx.saved_tensors
+        return on_device(saved[0].get_device(), _backward, saved, ctx.needs_input_grad, ctx.how, dh, dn)
 
 
 def _check(y, residual, weight, gate, next_weight, quant, what):
     if not y.is_cuda:
         raise RuntimeError(f"{what} runs on a CUDA device only (sm_100a); there is no CPU path")
-    if y.dtype not in ROW_TYPES:
+    dtype = y.dtype
+    if dtype not in ROW_TYPES:
         raise TypeError("rows must be bfloat16, float16 or float32")
-    H = y.shape[-1] if y.dim() else 0
+    shape = y.shape
+    H = shape[-1] if shape else 0
     if not 1 <= H <= MAX_ROW:
         raise ValueError(f"rows must have 1 to {MAX_ROW} values")
-    if quant not in (None, "int8"):
+    if quant is not None and quant != "int8":
         raise ValueError(f"quant={quant!r}: None or 'int8'")
-    if residual is not None and (residual.shape != y.shape or residual.dtype != y.dtype):
-        raise ValueError("residual must have the rows' shape and type")
-    for name, w in (("weight", weight), ("next_weight", next_weight)):
-        if w is not None and (w.dim() != 1 or w.shape[0] != H or w.dtype not in (y.dtype, torch.float32)):
-            raise ValueError(f"{name} must hold {H} values of the rows' type or float32")
+    index = y.get_device()
+    grad, away = y.requires_grad, False
+    if residual is not None:
+        if residual.dtype is not dtype or residual.shape != shape:
+            raise ValueError("residual must have the rows' shape and type")
+        grad |= residual.requires_grad
+        away |= residual.get_device() != index
+    for w in (weight, next_weight):
+        if w is not None:
+            if w.dim() != 1 or w.shape[0] != H or (w.dtype is not dtype and w.dtype is not _F32):
+                raise ValueError(f"weights must hold {H} values of the rows' type or float32")
+            grad |= w.requires_grad
+            away |= w.get_device() != index
     kind = _lib.GATE_NONE
     if gate is not None:
-        if gate.dtype not in (y.dtype, torch.float32):
+        if gate.dtype is not dtype and gate.dtype is not _F32:
             raise TypeError("gate must be of the rows' type or float32")
         if gate.dim() == 1 and gate.shape[0] == H:
             kind = _lib.GATE_CHANNEL
-        elif gate.shape == (*y.shape[:-1], 1):
-            kind = _lib.GATE_TOKEN
-        elif gate.shape == y.shape:
+        elif gate.shape == shape:
             kind = _lib.GATE_FULL
+        elif gate.shape == (*shape[:-1], 1):
+            kind = _lib.GATE_TOKEN
         else:
             raise ValueError(f"gate must be [{H}], [..., 1] or [..., {H}] over the rows' leading sizes")
-    for t in (residual, weight, gate, next_weight):
-        if t is not None and t.device != y.device:
-            raise ValueError("all tensors must be on one device")
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, residual, weight, gate, next_weight))
+        grad |= gate.requires_grad
+        away |= gate.get_device() != index
+    if away:
+        raise ValueError("all tensors must be on one device")
+    grad = grad and torch.is_grad_enabled()
     if grad and quant:
         raise RuntimeError("8-bit rows have no gradient: call it under torch.no_grad()")
     return kind, grad
@@ -156,14 +167,12 @@ def fused_pre_norm(x, weight, *, residual=None, eps=1e-6, quant=None):
     kind, grad = _check(x, residual, None, None, weight, quant, "fused_pre_norm")
     want_h = residual is not None
     if grad:
-        h, n = _BlockNorm.apply(x, residual, None, None, weight, kind, 1.0, float(eps), want_h)
+        h, n = _BlockNorm.apply(x, residual, None, None, weight, (kind, 1.0), float(eps), want_h)
         return (n, h) if want_h else n
-    with on_device(x):
-        h, n, q, scale, _ = _forward(x, residual, None, None, kind, weight, 1.0, eps, want_h, quant, False)
-    out = (q, scale) if quant else (n,)
-    if want_h:
-        out = (*out, h)
-    return out if len(out) > 1 else n
+    h, n, q, scale, _ = on_device(x.get_device(), _forward, x, residual, None, None, kind, weight, 1.0, eps, want_h, quant, False)
+    if quant:
+        return (q, scale, h) if want_h else (q, scale)
+    return (n, h) if want_h else n
 
 
 def fused_post_norm(y, residual, weight=None, *, gate=None, residual_scale=1.0, eps=1e-6, next_weight=None, quant=None):
@@ -184,8 +193,7 @@ def fused_post_norm(y, residual, weight=None, *, gate=None, residual_scale=1.0, 
         raise ValueError("quant belongs to the next block's input norm: pass next_weight")
     alpha = float(residual_scale)
     if grad:
-        h, n = _BlockNorm.apply(y, residual, weight, gate, next_weight, kind, alpha, float(eps), True)
+        h, n = _BlockNorm.apply(y, residual, weight, gate, next_weight, (kind, alpha), float(eps), True)
         return h if next_weight is None else (h, n)
-    with on_device(y):
-        h, n, q, scale, _ = _forward(y, residual, weight, gate, kind, next_weight, alpha, eps, True, quant, False)
+    h, n, q, scale, _ = on_device(y.get_device(), _forward, y, residual, weight, gate, kind, next_weight, alpha, eps, True, quant, False)
     return (h, q, scale) if quant else h if next_weight is None else (h, n)

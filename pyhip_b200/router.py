@@ -28,14 +28,20 @@ class RouterOutput(NamedTuple):
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(T, E, S):
+def _layout(T, E, S):
+    """Byte sizes: the launch's workspace; what the backward pass needs (lse [2, T], seg [T], coef [S, E], stats [2] in a row)."""
     b = ctypes.c_int64()
     _lib.check(_lib.lib().b200moe_router_workspace(T, E, S, ctypes.byref(b)), "router_workspace")
-    return b.value
+    return b.value, 4 * (3 * T + S * E + 2)
 
 
 def _p(t):
     return None if t is None else t.data_ptr()
+
+
+def _saved_at(saved, T, S, E):
+    lse = saved.data_ptr()
+    return lse, lse + 8 * T, lse + 12 * T, lse + 12 * T + 4 * S * E
 
 
 def _forward(logits, K, scoring, renorm, mask, cu, save):
@@ -43,34 +49,44 @@ def _forward(logits, K, scoring, renorm, mask, cu, save):
     T, E = x.shape
     dev = x.device
     S = 1 if cu is None else cu.shape[0] - 1
-    weights = torch.empty(T, K, dtype=torch.float32, device=dev)
-    ids = torch.empty(T, K, dtype=torch.int32, device=dev)
+    work, keep = _layout(T, E, S)
+    weights = torch.empty((T, K), dtype=torch.float32, device=dev)
+    ids = torch.empty((T, K), dtype=torch.int32, device=dev)
     counts = torch.empty((E,) if cu is None else (S, E), dtype=torch.int32, device=dev)
     balance = torch.empty((), dtype=torch.float32, device=dev)
     z = torch.empty((), dtype=torch.float32, device=dev)
-    size = _workspace_bytes(T, E, S)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    lse = seg = coef = stats = None
+    ws = torch.empty(work, dtype=torch.uint8, device=dev)
+    saved, at = None, (None, None, None, None)
     if save:
-        lse = torch.empty(2, T, dtype=torch.float32, device=dev)
-        seg = torch.empty(T, dtype=torch.int32, device=dev)
-        coef = torch.empty(S, E, dtype=torch.float32, device=dev)
-        stats = torch.empty(2, dtype=torch.float32, device=dev)
+        saved = torch.empty(keep, dtype=torch.uint8, device=dev)
+        at = _saved_at(saved, T, S, E)
     _lib.check(_lib.lib().b200moe_router_forward(
         x.data_ptr(), stride, T, E, K, ROW_TYPES[x.dtype], scoring, renorm, _p(mask), _p(cu), S, weights.data_ptr(),
-        ids.data_ptr(), counts.data_ptr(), balance.data_ptr(), z.data_ptr(), _p(lse), _p(seg), _p(coef), _p(stats), ws.data_ptr(),
-        size, stream_of(x)), "router_forward")
-    return weights, ids, counts, balance, z, (x, lse, seg, coef, stats)
+        ids.data_ptr(), counts.data_ptr(), balance.data_ptr(), z.data_ptr(), *at, ws.data_ptr(), work,
+        stream_of(x.get_device())), "router_forward")
+    return weights, ids, counts, balance, z, saved
+
+
+def _backward(logits, weights, ids, saved, how, dweights, dbalance, dz):
+    K, scoring, renorm, S = how
+    x, stride = rows_of(logits)
+    T, E = x.shape
+    if dweights is not None:
+        dweights = dweights.contiguous()
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _lib.check(_lib.lib().b200moe_router_backward(
+        x.data_ptr(), stride, T, E, K, ROW_TYPES[x.dtype], scoring, renorm, *_saved_at(saved, T, S, E), ids.data_ptr(),
+        weights.data_ptr(), _p(dweights), _p(dbalance), _p(dz), out.data_ptr(), stream_of(x.get_device())), "router_backward")
+    return out, None, None, None, None, None
 
 
 class _Router(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, K, scoring, renorm, mask, cu):
-        with on_device(logits):
-            weights, ids, counts, balance, z, (x, lse, seg, coef, stats) = _forward(logits, K, scoring, renorm, mask, cu, True)
+        weights, ids, counts, balance, z, saved = on_device(logits.get_device(), _forward, logits, K, scoring, renorm, mask, cu, True)
         # the rows that the backward pass reads are the input itself: saved as such, so that a change in place is noticed
-        ctx.save_for_backward(logits, weights, ids, lse, seg, coef, stats)
-        ctx.how = (K, scoring, renorm)
+        ctx.save_for_backward(logits, weights, ids, saved)
+        ctx.how = (K, scoring, renorm, 1 if cu is None else cu.shape[0] - 1)
         ctx.mark_non_differentiable(ids, counts)
         ctx.set_materialize_grads(False)
         return weights, ids, counts, balance, z
@@ -78,18 +94,8 @@ class _Router(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dweights, _ids, _counts, dbalance, dz):
-        logits, weights, ids, lse, seg, coef, stats = ctx.saved_tensors
-        K, scoring, renorm = ctx.how
-        with on_device(logits):
-            x, stride = rows_of(logits)
-            T, E = x.shape
-            dweights = None if dweights is None else dweights.contiguous()
-            out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            _lib.check(_lib.lib().b200moe_router_backward(
-                x.data_ptr(), stride, T, E, K, ROW_TYPES[x.dtype], scoring, renorm, lse.data_ptr(), seg.data_ptr(),
-                coef.data_ptr(), stats.data_ptr(), ids.data_ptr(), weights.data_ptr(), _p(dweights), _p(dbalance), _p(dz),
-                out.data_ptr(), stream_of(x)), "router_backward")
-        return out, None, None, None, None, None
+        logits, weights, ids, saved = ctx.saved_tensors
+        return on_device(logits.get_device(), _backward, logits, weights, ids, saved, ctx.how, dweights, dbalance, dz)
 
 
 def fused_router(gating_output, topk: int, *, renormalize: bool = True, scoring: str = "softmax", token_mask=None,
@@ -133,5 +139,4 @@ def fused_router(gating_output, topk: int, *, renormalize: bool = True, scoring:
     args = (int(topk), _SCORING[scoring], 1 if renormalize else 0, token_mask, cu_seqlens)
     if gating_output.requires_grad and torch.is_grad_enabled():
         return RouterOutput(*_Router.apply(gating_output, *args))
-    with on_device(gating_output):
-        return RouterOutput(*_forward(gating_output, *args, False)[:5])
+    return RouterOutput(*on_device(gating_output.get_device(), _forward, gating_output, *args, False)[:5])
