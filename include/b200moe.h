@@ -325,10 +325,11 @@ int b200moe_quantize_int8(const void* x, int64_t x_stride, int32_t T, int32_t K,
 /* W8A8 linear layer: y[t,n] = (sum_k q[t,k] weight[n,k]) * scale[t] * weight_scale[n] + bias[n], the sum exact in int32,
  * rounded once to out_dtype (bf16 or fp16).  K a multiple of 16 below 2^17 (up to 16384 for rows quantised here).
  *   x          i8 [T, K] (x_dtype INT8, x_stride = K, with x_scale [T]) or bf16 / fp16 / fp32 rows, which are quantised
- *              first into workspace (round_up(T*K, 256) + 4 T bytes, 16-byte aligned; unused for INT8)
+ *              first into workspace (b200moe_linear_int8_workspace bytes, 16-byte aligned; unused for INT8)
  *   weight     i8 [N, K], 16-byte aligned;  weight_scale f32 [N];  bias f32 [N] or NULL
  *   variant    0 = by size, 1 = split-K tiles for few tokens, 2 = CTA pairs
  *   status     i32 [2] or NULL: word 0 = id of a bounded wait that ran out (left alone otherwise), word 1 = CTA */
+int b200moe_linear_int8_workspace(int32_t T, int32_t N, int32_t K, int32_t variant, int64_t* bytes);
 int b200moe_linear_int8(const void* x, int64_t x_stride, int32_t x_dtype, const float* x_scale, const void* weight,
                         const float* weight_scale, const float* bias, int32_t T, int32_t N, int32_t K, int32_t out_dtype,
                         int32_t variant, void* workspace, int64_t workspace_bytes, int32_t* status, void* y, void* stream);

@@ -5,6 +5,8 @@ raw device pointers and the current torch stream passed as ``void*``
 (src/core/hiptools.py:10-35,82-100 of tingqli/pyhip); a non-zero status becomes a Python
 exception, as the reference's ``HIP error`` exceptions do (hiptools.py:37-39).
 
+The dense operators around the layer (`dense()`) are reached through a torch binding that calls the same C ABI.
+
 There is no fallback: if the shared library is missing or fails to load, importing callers
 get an ImportError / RuntimeError that says how to build it.
 """
@@ -13,11 +15,13 @@ from __future__ import annotations
 import ctypes
 import functools
 import pathlib
+import shutil
 import subprocess
 
 PKG_DIR = pathlib.Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libb200moe.so"
+DENSE_PATH = PKG_DIR / "_dense.so"          # torch binding of the dense operators (csrc/dense_torch.cpp)
 SOURCES = ["api.cu", "moe_aux.cu", "moe_gemm_sm100.cu", "moe_gemm_fp8_sm100.cu", "moe_gemm_bf16_sm100.cu",
            "moe_batch1.cu", "forward_static.cu", "block_norm.cu", "router_train.cu", "linear_int8_sm100.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -64,26 +68,47 @@ EXPORTS = ["b200moe_version", "b200moe_last_error", "b200moe_workspace_layout",
            "b200moe_sort_scratch_bytes", "b200moe_route_topk", "b200moe_forward_static", "b200moe_gather_sum", "b200moe_debug_probe",
            "b200moe_forward_ex", "b200moe_static_status", "b200moe_ep_plan", "b200moe_quant_rows_fp8_1x128",
            "b200moe_forward_batch1", "b200moe_batch1_scratch_bytes",
-           "b200moe_quantize_int8", "b200moe_linear_int8", "b200moe_block_norm", "b200moe_block_norm_bwd",
+           "b200moe_quantize_int8", "b200moe_linear_int8", "b200moe_linear_int8_workspace", "b200moe_block_norm", "b200moe_block_norm_bwd",
            "b200moe_block_norm_bwd_workspace", "b200moe_router_workspace", "b200moe_router_forward",
            "b200moe_router_backward"]
 
 
+def _stale(target, deps) -> bool:
+    return not target.exists() or any(target.stat().st_mtime < d.stat().st_mtime for d in deps)
+
+
+def _dense_command():
+    import sysconfig
+
+    import torch
+    root = pathlib.Path(torch.__file__).resolve().parent
+    cuda = pathlib.Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve().parents[1]
+    inc = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], cuda / "include"]
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_dense",
+            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(f"-isystem{i}" for i in inc), "-o", str(DENSE_PATH), str(CSRC / "dense_torch.cpp"), f"-L{root / 'lib'}", "-lc10",
+            "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", f"-L{PKG_DIR}", "-l:libb200moe.so", "-Wl,-rpath,$ORIGIN",
+            f"-Wl,-rpath,{root / 'lib'}"]
+
+
 def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
     """Compile the CUDA sources for sm_100a into pyhip_b200/libb200moe.so (nvcc cross-compiles
-    without a GPU)."""
+    without a GPU) and the torch binding of the dense operators into pyhip_b200/_dense.so."""
+    header = PKG_DIR.parent / "include" / "b200moe.h"
     srcs = [CSRC / s for s in SOURCES]
-    deps = srcs + list(CSRC.glob("*.h")) + list(CSRC.glob("*.cuh")) + [PKG_DIR.parent / "include" / "b200moe.h"]
-    if not force and LIB_PATH.exists() and all(LIB_PATH.stat().st_mtime >= d.stat().st_mtime for d in deps):
-        return LIB_PATH
-    cmd = ["nvcc", *NVCC_FLAGS, "-o", str(LIB_PATH), *map(str, srcs)]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-    if verbose:
-        print(res.stderr)
+    if force or _stale(LIB_PATH, srcs + list(CSRC.glob("*.h")) + list(CSRC.glob("*.cuh")) + [header]):
+        cmd = ["nvcc", *NVCC_FLAGS, "-o", str(LIB_PATH), *map(str, srcs)]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+        if verbose:
+            print(res.stderr)
+    if force or _stale(DENSE_PATH, [CSRC / "dense_torch.cpp", header]):
+        res = subprocess.run(_dense_command(), capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("g++ failed:\n" + res.stdout + res.stderr)
     return LIB_PATH
 
 
@@ -125,6 +150,7 @@ def lib() -> ctypes.CDLL:
     norm = [vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, i32, i32, i32, f32]
     L.b200moe_quantize_int8.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp]
     L.b200moe_linear_int8.argtypes = [vp, i64, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, vp, vp, vp]
+    L.b200moe_linear_int8_workspace.argtypes = [i32, i32, i32, i32, ctypes.POINTER(i64)]
     L.b200moe_block_norm.argtypes = norm + [f32] + [vp] * 6
     L.b200moe_block_norm_bwd.argtypes = norm + [vp] * 8 + [vp, i64, vp]
     L.b200moe_block_norm_bwd_workspace.argtypes = [i32, i32, i32, ctypes.POINTER(i64)]
@@ -141,6 +167,22 @@ def lib() -> ctypes.CDLL:
 
 class B200MoEError(RuntimeError):
     pass
+
+
+@functools.cache
+def dense():
+    """The torch binding of the dense operators.  Like `lib()` it has no fallback."""
+    lib()                                   # the library that it links against, of the version that it was built for
+    if not DENSE_PATH.exists():
+        raise ImportError(f"{DENSE_PATH} is missing: run `python -c 'import __graft_entry__ as g; g.build()'`")
+    import importlib.util
+
+    import torch  # noqa: F401  (its libraries have to be loaded first)
+    spec = importlib.util.spec_from_file_location("pyhip_b200._dense", DENSE_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.set_error(B200MoEError)
+    return module
 
 
 def check(rc: int, what: str) -> None:

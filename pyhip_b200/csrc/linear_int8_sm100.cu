@@ -574,6 +574,12 @@ int launch_linear_int8(const void* q, const float* x_scale, const void* w, const
 
 using namespace b200moe;
 
+extern "C" int b200moe_linear_int8_workspace(int32_t T, int32_t N, int32_t K, int32_t variant, int64_t* bytes) {
+  B200_CHECK_ARG(bytes != nullptr && T >= 0 && N >= 1 && K >= 1 && variant >= 0 && variant <= 2, "linear_int8_workspace: T=%d N=%d K=%d", T, N, K);
+  *bytes = T == 0 ? 0 : round_up64((int64_t)T * K, 256) + (int64_t)T * 4;     // the quantised rows and their scales
+  return 0;
+}
+
 extern "C" int b200moe_linear_int8(const void* x, int64_t x_stride, int32_t x_dtype, const float* x_scale, const void* weight,
                                    const float* weight_scale, const float* bias, int32_t T, int32_t N, int32_t K, int32_t out_dtype,
                                    int32_t variant, void* workspace, int64_t workspace_bytes, int32_t* status, void* y, void* stream) {

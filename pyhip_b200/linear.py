@@ -9,7 +9,7 @@ rows the GEMM stores in sorted order are already the result.  Same kernels, same
 C ABI calls (`b200moe_sort_align`, `b200moe_quant_rows[_e4m3]`, `b200moe_down`).
 
 `linear_int8` is the product of 8-bit integers with one scale per token and per output channel, which the reference does not
-have: its C ABI call (`b200moe_linear_int8`) quantises the tokens and multiplies, two launches.
+have: one C ABI call (`b200moe_linear_int8`) quantises the tokens and multiplies.
 """
 from __future__ import annotations
 
@@ -19,7 +19,6 @@ import torch
 
 from . import _lib
 from .fused_moe import _capacity, _ptr, _stream, get_plan, pick_block
-from .rows import MAX_ROW, ROW_TYPES, on_device, rows_of, stream_of
 
 
 class PreparedLinear:
@@ -115,47 +114,15 @@ def quantize_int8(x):
     scale = max(max |x| / 127, 2**-100) and q the whole number nearest to x / scale (ties to even, decided exactly).
     The activation format of `linear_int8`; with rows as output channels it also makes that layer's weights.
     A row that holds an infinity or NaN gets scale NaN.  K <= 16384.  There is no gradient."""
-    if not x.is_cuda:
-        raise RuntimeError("quantize_int8 runs on a CUDA device only (sm_100a); there is no CPU path")
-    dt = ROW_TYPES.get(x.dtype)
-    if dt is None:
-        raise TypeError("x must be bfloat16, float16 or float32")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_ROW:
-        raise ValueError(f"rows of x must have 1 to {MAX_ROW} values")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("quantize_int8 has no gradient: call it under torch.no_grad() or on a detached tensor")
-    return on_device(x.get_device(), _quantize_int8, x, dt)
-
-
-def _quantize_int8(x, dt):
-    x2, stride = rows_of(x)
-    T, K = x2.shape
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _lib.check(_lib.lib().b200moe_quantize_int8(x2.data_ptr(), stride, T, K, dt, q.data_ptr(), scale.data_ptr(),
-                                                stream_of(x.get_device())), "quantize_int8")
-    return q, scale
-
-
-_int8_status: dict = {}
+    return _lib.dense().quantize_int8(x)
 
 
 def int8_status(device=None):
     """Host read of the error words that `linear_int8` calls on ``device`` leave (synchronises; for tests and debugging):
     (id of the barrier wait that ran out, its CTA), (0, 0) if none ever did."""
-    index = torch.cuda.current_device() if device is None else torch.device(device).index
-    t = _int8_status.get(torch.cuda.current_device() if index is None else index)
-    return (0, 0) if t is None else tuple(t[0].cpu().tolist())
-
-
-def _status_words(index):
-    """(tensor, address) of the device's status words, or an address of None where a graph that is being captured would have to
-    hold them: its memory would not outlive it."""
-    if torch.cuda.is_current_stream_capturing():
-        return None, None
-    t = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", index))
-    _int8_status[index] = (t, t.data_ptr())
-    return _int8_status[index]
+    index = None if device is None else torch.device(device).index
+    t = _lib.dense().int8_status(torch.cuda.current_device() if index is None else index)
+    return (0, 0) if t is None else tuple(t.cpu().tolist())
 
 
 def linear_int8(x, weight, weight_scale, *, x_scale=None, bias=None, out_dtype=None, variant: int = 0):
@@ -170,71 +137,4 @@ def linear_int8(x, weight, weight_scale, *, x_scale=None, bias=None, out_dtype=N
       ``variant``: 0 chooses the kernel by size, 1 = split-K tiles for few tokens, 2 = CTA pairs
 
     K must be a multiple of 16 below 2**17.  There is no gradient.  Returns [..., N]."""
-    if not x.is_cuda:
-        raise RuntimeError("linear_int8 runs on a CUDA device only (sm_100a); there is no CPU path")
-    index = x.get_device()
-    if weight.dtype is not torch.int8 or weight.dim() != 2:
-        raise TypeError("weight must be an int8 matrix [N, K]")
-    N, K = weight.shape
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise ValueError(f"x has shape {tuple(x.shape)}, the weight {K} columns")
-    if N < 1 or K < 16 or K % 16 or K >= 1 << 17:
-        raise ValueError(f"weight [{N}, {K}]: K must be a multiple of 16 below 2**17")
-    if weight_scale.dtype is not torch.float32 or weight_scale.numel() != N:
-        raise ValueError("weight_scale must hold one float32 scale per output channel")
-    if bias is not None and (bias.dtype is not torch.float32 or bias.numel() != N):
-        raise ValueError("bias must hold one float32 value per output channel")
-    dt = ROW_TYPES.get(x.dtype)
-    if dt is not None:
-        if x_scale is not None:
-            raise ValueError("x_scale belongs to int8 rows")
-        if K > MAX_ROW:
-            raise ValueError(f"rows that are quantised here have up to {MAX_ROW} values")
-    elif x.dtype is torch.int8:
-        dt = _lib.T_INT8
-        if x_scale is None or x_scale.dtype is not torch.float32 or x_scale.shape != x.shape[:-1]:
-            raise ValueError("int8 rows need x_scale, one float32 per row")
-    else:
-        raise TypeError("x must be int8, bfloat16, float16 or float32")
-    if (weight.get_device() != index or weight_scale.get_device() != index or (bias is not None and bias.get_device() != index)
-            or (x_scale is not None and x_scale.get_device() != index)):
-        raise ValueError("all tensors must be on one device")
-    if (x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad) or
-            (x_scale is not None and x_scale.requires_grad)) and torch.is_grad_enabled():
-        raise RuntimeError("linear_int8 has no gradient: call it under torch.no_grad() or on detached tensors")
-    if out_dtype is None:
-        out_dtype = x.dtype if dt < _lib.T_FP32 else torch.bfloat16
-    elif out_dtype is not torch.bfloat16 and out_dtype is not torch.float16:
-        raise TypeError("out_dtype must be bfloat16 or float16")
-    if variant not in (0, 1, 2):
-        raise ValueError(f"variant={variant!r}: 0, 1 or 2")
-    return on_device(index, _linear_int8, x, weight, weight_scale, x_scale, bias, out_dtype, variant, dt, index)
-
-
-def _linear_int8(x, weight, weight_scale, x_scale, bias, out_dtype, variant, dt, index):
-    status = _int8_status.get(index)
-    if status is None:
-        status = _status_words(index)
-    N, K = weight.shape
-    x2, stride = rows_of(x)
-    T = x2.shape[0]
-    dev = x.device
-    y = torch.empty((T, N) if x.dim() == 2 else (*x.shape[:-1], N), dtype=out_dtype, device=dev)
-    ws = xs = None
-    need = 0
-    if dt == _lib.T_INT8:
-        if stride != K or x2.data_ptr() & 15:
-            x2, stride = x2.clone(memory_format=torch.contiguous_format), K
-        xs = x_scale.contiguous()
-    else:
-        need = (T * K + 255) // 256 * 256 + 4 * T
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    w = weight if weight.is_contiguous() and not weight.data_ptr() & 15 else weight.clone(memory_format=torch.contiguous_format)
-    sc = weight_scale.contiguous()
-    if bias is not None:
-        bias = bias.contiguous()
-    _lib.check(_lib.lib().b200moe_linear_int8(
-        x2.data_ptr(), stride, dt, None if xs is None else xs.data_ptr(), w.data_ptr(), sc.data_ptr(),
-        None if bias is None else bias.data_ptr(), T, N, K, ROW_TYPES[out_dtype], variant, None if ws is None else ws.data_ptr(), need,
-        status[1], y.data_ptr(), stream_of(index)), "linear_int8")
-    return y
+    return _lib.dense().linear_int8(x, weight, weight_scale, x_scale, bias, out_dtype, variant)
