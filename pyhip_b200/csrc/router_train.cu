@@ -42,11 +42,39 @@ struct RouterParams {
   int T, E, K, S, rows, scoring, renorm;
 };
 
-// ascending unsigned order = ascending float order; NaN above everything, the two zeros alike, 0 = taken
-__device__ __forceinline__ uint32_t order_key(float v) {
-  const uint32_t u = __float_as_uint(v + 0.f);
+// Order keys of the logits: ascending unsigned order = ascending float order, NaN above everything, the two zeros alike, and
+// 0 = taken (no value has it).  A 16-bit logit leaves room for its expert: one maximum then finds both, the lowest expert
+// first among equal logits; a 32-bit one needs a second reduction over the experts that hold the maximum.
+template <typename T> constexpr bool kKeyHoldsExpert = sizeof(T) == 2;
+__device__ __forceinline__ uint32_t order32(uint32_t u) {
   if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  if (u == 0x80000000u) u = 0u;
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ uint32_t order_key(float v, int) { return order32(__float_as_uint(v)); }
+__device__ __forceinline__ uint32_t order16(uint32_t u, uint32_t inf) {
+  if ((u & 0x7fffu) > inf) return 0xffffu;
+  if (u == 0x8000u) u = 0u;
+  return u ^ ((u >> 15) ? 0xffffu : 0x8000u);
+}
+__device__ __forceinline__ uint32_t order_key(__nv_bfloat16 v, int e) {
+  return (order16(__bfloat16_as_ushort(v), 0x7f80u) << 16) | (0xffffu - (uint32_t)e);
+}
+__device__ __forceinline__ uint32_t order_key(__half v, int e) {
+  return (order16(__half_as_ushort(v), 0x7c00u) << 16) | (0xffffu - (uint32_t)e);
+}
+// the logit of a key
+template <typename T> __device__ __forceinline__ float key_value(uint32_t k);
+template <> __device__ __forceinline__ float key_value<float>(uint32_t k) {
+  return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+template <> __device__ __forceinline__ float key_value<__nv_bfloat16>(uint32_t k) {
+  k >>= 16;
+  return __uint_as_float((k ^ ((k >> 15) ? 0x8000u : 0xffffu)) << 16);
+}
+template <> __device__ __forceinline__ float key_value<__half>(uint32_t k) {
+  k >>= 16;
+  return __half2float(__ushort_as_half((unsigned short)(k ^ ((k >> 15) ? 0x8000u : 0xffffu))));
 }
 template <int LPR>
 __device__ __forceinline__ float group_sum(float v) {
@@ -76,7 +104,23 @@ __device__ __forceinline__ float group_max_nan(float v) {
   for (int d = LPR / 2; d > 0; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;
 }
-__device__ __forceinline__ float log_sigmoid(float l) { return fminf(l, 0.f) - log1pf(expf(-fabsf(l))); }
+
+// A row's scores up to the factor exp(shift): softmax exp(l - max) with shift = max; sigmoid 1 / (1 + exp(-l)) with shift = 0,
+// or, where every logit is negative, exp(l - max) / (1 + exp(l)) with shift = max, which cannot underflow for all of them.
+struct RowScore {
+  float lmax;
+  bool sigmoid, shifted;
+  __device__ RowScore(float lmax_, bool sigmoid_) : lmax(lmax_), sigmoid(sigmoid_), shifted(!sigmoid_ || lmax_ < 0.f) {}
+  __device__ __forceinline__ float shift() const { return shifted ? lmax : 0.f; }
+  // score of l, and exp(l - max) in `el`
+  __device__ __forceinline__ float operator()(float l, float& el) const {
+    el = expf(l - lmax);
+    if (!sigmoid) return el;
+    if (shifted) return __fdividef(el, 1.f + expf(l));
+    const float t = expf(-fabsf(l));
+    return __fdividef(l >= 0.f ? 1.f : t, 1.f + t);
+  }
+};
 
 __device__ __forceinline__ int clamp_row(int v, int T) { return min(max(v, 0), T); }
 
@@ -127,63 +171,67 @@ router_forward_kernel(const __grid_constant__ RouterParams p) {
     for (int tb = at + warp * RPW; tb < end; tb += kRouterWarps * RPW) {     // uniform in the warp
       const int t = tb + sub;
       const bool row = t < end;
-      bool live = row && (p.mask == nullptr || p.mask[t] != 0);
       const T* src = static_cast<const T*>(p.logits) + (int64_t)t * p.stride;
-      float l[VPL];
+      float l[VPL], ex[VPL];
       uint32_t key[VPL];
       float lmax = -INFINITY;
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
         const int e = l0 + i * LPR;
-        const bool in = live && e < E;
-        l[i] = in ? to_f(src[e]) : -INFINITY;
-        key[i] = in ? order_key(l[i]) : 0u;
+        const bool in = row && e < E;
+        const T v = in ? src[e] : from_f<T>(-INFINITY);
+        l[i] = to_f(v);
+        key[i] = in ? order_key(v, e) : 0u;
         lmax = max_nan(lmax, l[i]);
       }
+      bool live = row && (p.mask == nullptr || p.mask[t] != 0);
       lmax = group_max_nan<LPR>(lmax);
       live = live && lmax != -INFINITY;
-      float ex[VPL], amax = lmax, sum = 0.f, sum_l = 0.f;
-      if (p.scoring == 0) {
+      const RowScore score(lmax, p.scoring != 0);
+      float sum = 0.f, sum_l = 0.f;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) { ex[i] = expf(l[i] - amax); sum += ex[i]; }
-        sum = group_sum<LPR>(sum);
-      } else {
-        amax = log_sigmoid(lmax);
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-          ex[i] = expf(log_sigmoid(l[i]) - amax);
-          sum += ex[i];
-          sum_l += expf(l[i] - lmax);
-        }
-        sum = group_sum<LPR>(sum);
-        sum_l = group_sum<LPR>(sum_l);
+      for (int i = 0; i < VPL; ++i) {
+        float el;
+        ex[i] = score(l[i], el);
+        sum += ex[i];
+        sum_l += el;
       }
+      sum = group_sum<LPR>(sum);
+      sum_l = p.scoring == 0 ? sum : group_sum<LPR>(sum_l);
       const float inv = 1.f / sum;
-      const float lse_a = amax + logf(sum), lse_l = p.scoring == 0 ? lse_a : lmax + logf(sum_l);
+      const float lse_a = score.shift() + logf(sum), lse_l = lmax + logf(sum_l);
       // lane k of the row keeps the k-th choice
-      float chosen = 0.f, total = 0.f;
+      uint32_t my_key = 0u;
       int id = 0;
       for (int k = 0; k < K; ++k) {
         uint32_t best = key[0];
 #pragma unroll
         for (int i = 1; i < VPL; ++i) best = max(best, key[i]);
         best = group_max<LPR>(best);
-        uint32_t mine = 0x7fffffffu;                     // lowest expert of this lane that holds the best key
+        int e;
+        if constexpr (kKeyHoldsExpert<T>) {
+          e = (int)(0xffffu - (best & 0xffffu));
 #pragma unroll
-        for (int i = VPL - 1; i >= 0; --i)
-          if (key[i] == best) mine = (uint32_t)(l0 + i * LPR);
-        const uint32_t e = group_min<LPR>(mine);
-        float v = 0.f;
+          for (int i = 0; i < VPL; ++i) key[i] = key[i] == best ? 0u : key[i];
+        } else {
+          uint32_t mine = 0x7fffffffu;                   // lowest expert of this lane that holds the best key
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-          if (e == (uint32_t)(l0 + i * LPR)) { v = ex[i]; key[i] = 0u; }
-        v = __shfl_sync(0xffffffffu, v, (int)(e % LPR), LPR);
-        total += v;
-        if (l0 == k) { chosen = v; id = (int)e; }
+          for (int i = VPL - 1; i >= 0; --i)
+            if (key[i] == best) mine = (uint32_t)(l0 + i * LPR);
+          const uint32_t first = group_min<LPR>(mine);
+          e = (int)first;
+#pragma unroll
+          for (int i = 0; i < VPL; ++i)
+            if (first == (uint32_t)(l0 + i * LPR)) key[i] = 0u;
+        }
+        if (l0 == k) { my_key = best; id = e; }
       }
+      float chosen = 0.f, unused;
+      if (l0 < K) chosen = score(key_value<T>(my_key), unused);
+      const float total = group_sum<LPR>(chosen);
       if (live) {
         if (l0 < K) {
-          const float w = p.renorm ? chosen / total : (p.scoring == 0 ? chosen * inv : chosen * expf(amax));
+          const float w = p.renorm ? chosen / total : (p.scoring == 0 ? chosen * inv : chosen * expf(score.shift()));
           p.ids[(int64_t)t * K + l0] = id;
           p.weights[(int64_t)t * K + l0] = w;
           atomicAdd(&cnt[id], 1);
@@ -238,22 +286,23 @@ struct RouterJoinParams {
   int32_t* ticket;
   int32_t* counts;            // [S, E]
   float* coef;                // [S, E]: E counts / (K n_s^2), the loss of the sequence = sum(coef * sum of p)
-  float* seq;                 // [S, 3]: loss, live tokens, sum of logsumexp^2
+  float* seq;                 // [S, blocks, 3]: loss of the block's experts, live tokens, sum of logsumexp^2
   float* stats;               // {1 / sequences with live tokens, 1 / live tokens}
   float* balance; float* z;
   int T, E, K, S, rows, chunks;
 };
 
-// One CTA per sequence; the last one to finish joins the sequences in order.
-__global__ void __launch_bounds__(1024)
+// One CTA per sequence and 64 experts; the last one to finish joins the sequences in order.
+constexpr int kJoinThreads = 1024, kJoinCols = 64;
+__global__ void __launch_bounds__(kJoinThreads)
 router_join_kernel(const __grid_constant__ RouterJoinParams p) {
-  extern __shared__ float smem[];                       // [groups][E] sums of p, then the same of counts
-  __shared__ float red[32];
-  __shared__ float zs;
+  __shared__ float gp[kJoinThreads];                    // [groups][columns] sums of p, and of counts
+  __shared__ int32_t gc[kJoinThreads];
+  __shared__ float zs, half;
   __shared__ int ns, last;
   grid_dep_wait();
   grid_dep_launch();
-  const int s = blockIdx.x, E = p.E;
+  const int s = blockIdx.x, E = p.E, e0 = blockIdx.y * kJoinCols, nb = gridDim.y;
   int lo = 0, hi = p.T;
   if (p.cu != nullptr) {
     lo = clamp_row(p.cu[s], p.T);
@@ -261,70 +310,71 @@ router_join_kernel(const __grid_constant__ RouterJoinParams p) {
   }
   const int c0 = hi > lo ? lo / p.rows : 0, c1 = hi > lo ? (hi - 1) / p.rows + 1 : 0;
   // groups of threads take interleaved slots of a column; their sums are added in order
-  const int cols = min(E, (int)blockDim.x), groups = (int)blockDim.x / cols;
-  const int g = threadIdx.x / cols;
-  float* gp = smem;
-  int32_t* gc = reinterpret_cast<int32_t*>(smem + groups * E);
-  if (g < groups)
-    for (int e = threadIdx.x % cols; e < E; e += cols) {
-      float v = 0.f;
-      int c = 0;
+  const int cols = min(E - e0, kJoinCols), groups = kJoinThreads / cols;
+  const int g = threadIdx.x / cols, e = e0 + threadIdx.x % cols;
+  if (g < groups) {
+    float v = 0.f;
+    int c = 0;
 #pragma unroll 4
-      for (int i = c0 + g; i < c1; i += groups) {
-        v += p.part_p[(int64_t)(i + s) * E + e];
-        c += p.part_c[(int64_t)(i + s) * E + e];
-      }
-      gp[g * E + e] = v;
-      gc[g * E + e] = c;
+    for (int i = c0 + g; i < c1; i += groups) {
+      v += p.part_p[(int64_t)(i + s) * E + e];
+      c += p.part_c[(int64_t)(i + s) * E + e];
     }
-  if (threadIdx.x < 32) {
+    gp[threadIdx.x] = v;
+    gc[threadIdx.x] = c;
+  }
+  if (threadIdx.x >= kJoinThreads - 32) {
+    const int lane = threadIdx.x & 31;
     float z = 0.f;
     int n = 0;
-    for (int i = c0 + threadIdx.x; i < c1; i += 32) { z += p.part_z[i + s]; n += p.part_n[i + s]; }
+#pragma unroll 4
+    for (int i = c0 + lane; i < c1; i += 32) { z += p.part_z[i + s]; n += p.part_n[i + s]; }
     z = warp_sum(z);
     n = __reduce_add_sync(0xffffffffu, n);
-    if (threadIdx.x == 0) { zs = z; ns = n; }
+    if (lane == 0) { zs = z; ns = n; }
   }
   __syncthreads();
+  if (threadIdx.x >= kJoinCols) return;
   const float n = (float)ns;
   const float f = ns > 0 ? (float)E / ((float)p.K * n * n) : 0.f;
   float loss = 0.f;
-  for (int e = threadIdx.x; e < E; e += blockDim.x) {
+  if ((int)threadIdx.x < cols) {
     float v = 0.f;
     int c = 0;
-    for (int i = 0; i < groups; ++i) { v += gp[i * E + e]; c += gc[i * E + e]; }
+    for (int i = 0; i < groups; ++i) { v += gp[i * cols + threadIdx.x]; c += gc[i * cols + threadIdx.x]; }
     const float cf = f * (float)c;
     p.counts[(int64_t)s * E + e] = c;
     if (p.coef != nullptr) p.coef[(int64_t)s * E + e] = cf;
-    if (ns > 0) loss = fmaf(cf, v, loss);
+    if (ns > 0) loss = cf * v;
   }
   loss = warp_sum(loss);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = loss;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    loss = warp_sum(threadIdx.x < blockDim.x / 32 ? red[threadIdx.x] : 0.f);
-    if (threadIdx.x == 0) {
-      float* o = p.seq + (int64_t)s * 3;
-      o[0] = loss; o[1] = n; o[2] = zs;
-      __threadfence();
-      last = atomicAdd(p.ticket, 1) == (int)gridDim.x - 1;
-    }
-    __syncwarp();
-    if (last) {
-      __threadfence();
-      float tot = 0.f, tok = 0.f, z = 0.f, used = 0.f;
-      for (int i = threadIdx.x; i < p.S; i += 32) {
-        const volatile float* o = p.seq + (int64_t)i * 3;
-        tot += o[0]; tok += o[1]; z += o[2];
+  if (threadIdx.x == 32) half = loss;
+  asm volatile("bar.sync 1, 64;" ::: "memory");
+  if (threadIdx.x >= 32) return;
+  if (threadIdx.x == 0) {
+    float* o = p.seq + ((int64_t)s * nb + blockIdx.y) * 3;
+    o[0] = loss + half; o[1] = n; o[2] = zs;
+    __threadfence();
+    last = atomicAdd(p.ticket, 1) == (int)(gridDim.x * gridDim.y) - 1;
+  }
+  __syncwarp();
+  if (last) {
+    __threadfence();
+    float tot = 0.f, tok = 0.f, z = 0.f, used = 0.f;
+    for (int i = threadIdx.x; i < p.S * nb; i += 32) {
+      const volatile float* o = p.seq + (int64_t)i * 3;
+      tot += o[0];
+      if (i % nb == 0) {
+        tok += o[1]; z += o[2];
         used += o[1] > 0.f ? 1.f : 0.f;
       }
-      tot = warp_sum(tot); tok = warp_sum(tok); z = warp_sum(z); used = warp_sum(used);
-      if (threadIdx.x == 0) {
-        const float iu = 1.f / fmaxf(used, 1.f), it = 1.f / fmaxf(tok, 1.f);
-        *p.balance = tot * iu;
-        *p.z = z * it;
-        if (p.stats != nullptr) { p.stats[0] = iu; p.stats[1] = it; }
-      }
+    }
+    tot = warp_sum(tot); tok = warp_sum(tok); z = warp_sum(z); used = warp_sum(used);
+    if (threadIdx.x == 0) {
+      const float iu = 1.f / fmaxf(used, 1.f), it = 1.f / fmaxf(tok, 1.f);
+      *p.balance = tot * iu;
+      *p.z = z * it;
+      if (p.stats != nullptr) { p.stats[0] = iu; p.stats[1] = it; }
     }
   }
 }
@@ -345,12 +395,14 @@ struct RouterBwdParams {
 template <typename T, int LPR, int VPL>
 __global__ void __launch_bounds__(kRouterThreads)
 router_backward_kernel(const __grid_constant__ RouterBwdParams p) {
+  __shared__ float rows[kRouterWarps * (32 / LPR) * LPR * VPL];
   grid_dep_wait();
   grid_dep_launch();
   const int E = p.E, K = p.K;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane / LPR, l0 = lane % LPR;
   constexpr int RPW = 32 / LPR;
+  const bool sigmoid = p.scoring != 0;
   const float gb = p.dbalance != nullptr ? *p.dbalance * p.stats[0] : 0.f;
   const float gz = p.dz != nullptr ? 2.f * *p.dz * p.stats[1] : 0.f;
   for (int64_t tb = ((int64_t)blockIdx.x * kRouterWarps + warp) * RPW; tb < p.T; tb += (int64_t)gridDim.x * kRouterWarps * RPW) {
@@ -358,21 +410,16 @@ router_backward_kernel(const __grid_constant__ RouterBwdParams p) {
     const bool row = t < p.T;
     const int s = row ? p.seg[t] : -1;
     const bool live = s >= 0;
-    const float lse_a = live ? p.lse[t] : 0.f, lse_l = live ? p.lse[p.T + t] : 0.f;
     const T* src = static_cast<const T*>(p.logits) + t * p.stride;
-    float l[VPL], pr[VPL], q[VPL], dot = 0.f;
+    float l[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int e = l0 + i * LPR;
-      const bool in = live && e < E;
-      l[i] = in ? to_f(src[e]) : -INFINITY;
-      const float a = p.scoring == 0 ? l[i] : log_sigmoid(l[i]);
-      pr[i] = in ? expf(a - lse_a) : 0.f;
-      q[i] = (in && gb != 0.f) ? gb * p.coef[(int64_t)s * E + e] : 0.f;
-      dot = fmaf(pr[i], q[i], dot);
+      l[i] = row && e < E ? to_f(src[e]) : -INFINITY;
     }
-    // lane k of the row holds its k-th choice
-    float w = 0.f, dw = 0.f, wdw = 0.f;
+    // p = score / exp(lse - shift) as in the forward pass; m = d(a) / dl; pl = softmax(l)
+    const float lse_a = live ? p.lse[t] : 0.f, lse_l = live ? p.lse[p.T + t] : 0.f;
+    float w = 0.f, dw = 0.f, wdw = 0.f;                // lane k of the row holds its k-th choice
     int id = -1;
     if (live && l0 < K && p.dweights != nullptr) {
       w = p.weights[t * K + l0];
@@ -380,34 +427,52 @@ router_backward_kernel(const __grid_constant__ RouterBwdParams p) {
       id = p.ids[t * K + l0];
       wdw = w * dw;
     }
+    float pr[VPL], m[VPL], q[VPL], dot = 0.f;
+    const bool low = lse_a < -40.f;                    // sigmoid scores that may all underflow: in logarithms
+    const float scale = expf(-lse_a);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = l0 + i * LPR;
+      if (!sigmoid) {
+        pr[i] = expf(l[i] - lse_a);
+        m[i] = 1.f;
+      } else {
+        const float t1 = expf(-fabsf(l[i])), r = __fdividef(1.f, 1.f + t1);
+        pr[i] = low ? expf(l[i] - lse_a) * r : (l[i] >= 0.f ? r : t1 * r) * scale;
+        m[i] = l[i] >= 0.f ? t1 * r : r;
+      }
+      if (!live || e >= E) pr[i] = 0.f;
+      q[i] = (gb != 0.f && live && e < E) ? gb * p.coef[(int64_t)s * E + e] : 0.f;
+      dot = fmaf(pr[i], q[i], dot);
+    }
     dot = group_sum<LPR>(dot);
     const float sum_w = group_sum<LPR>(wdw);
     const float part = p.renorm ? w * (dw - sum_w) : wdw;
-    const float all = (!p.renorm && p.scoring == 0) ? dot + sum_w : dot;
+    const float all = (!p.renorm && !sigmoid) ? dot + sum_w : dot;
     float da[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) da[i] = pr[i] * (q[i] - all);
-    if (p.dweights != nullptr)
-      for (int k = 0; k < K; ++k) {
-        const int e = __shfl_sync(0xffffffffu, id, k, LPR);
-        const float v = __shfl_sync(0xffffffffu, part, k, LPR);
+    if (p.dweights != nullptr) {
+      // the choices' parts, by way of a row of zeros in shared memory
+      float* mine = rows + (warp * RPW + sub) * (LPR * VPL);
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-          if (e == l0 + i * LPR) da[i] += v;
-      }
+      for (int i = 0; i < VPL; ++i) mine[l0 + i * LPR] = 0.f;
+      __syncwarp();
+      if (id >= 0 && id < E) mine[id] = part;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) da[i] += mine[l0 + i * LPR];
+      __syncwarp();
+    }
     if (row) {
       T* dst = static_cast<T*>(p.dlogits) + t * E;
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
         const int e = l0 + i * LPR;
         if (e < E) {
-          float d = 0.f;
-          if (live) {
-            d = p.scoring == 0 ? da[i] : da[i] / (1.f + expf(l[i]));
-            const float pl = p.scoring == 0 ? pr[i] : expf(l[i] - lse_l);
-            d = fmaf(gz * lse_l, pl, d);
-          }
-          dst[e] = from_f<T>(d);
+          float d = da[i] * m[i];
+          if (gz != 0.f) d = fmaf(gz * lse_l, sigmoid ? expf(l[i] - lse_l) : pr[i], d);
+          dst[e] = from_f<T>(live ? d : 0.f);
         }
       }
     }
@@ -431,7 +496,7 @@ RouterLayout router_layout(int T, int E, int S) {
   r.off_z = r.off_c + pad(r.slots * E * 4);
   r.off_n = r.off_z + pad(r.slots * 4);
   r.off_seq = r.off_n + pad(r.slots * 4);
-  r.off_ticket = r.off_seq + pad((int64_t)S * 12);
+  r.off_ticket = r.off_seq + pad((int64_t)S * ((E + kJoinCols - 1) / kJoinCols) * 12);
   r.bytes = r.off_ticket + 256;
   return r;
 }
@@ -518,9 +583,7 @@ int b200moe_router_forward(const void* logits, int64_t stride, int32_t T, int32_
   }
   RouterJoinParams j = {cu_seqlens, p.part_p, p.part_c, p.part_z, p.part_n, p.ticket, counts, coef, (float*)(w + r.off_seq), stats,
                         balance_loss, z_loss, T, E, K, sequences, r.rows, r.chunks};
-  const int threads = sequences > 1 ? 256 : 1024;
-  const int cols = std::min((int)E, threads), groups = threads / cols;
-  B200_CHECK_CUDA(launch_chained(router_join_kernel, dim3(sequences), dim3(threads), (size_t)groups * E * 8, st, j));
+  B200_CHECK_CUDA(launch_chained(router_join_kernel, dim3(sequences, (E + kJoinCols - 1) / kJoinCols), dim3(kJoinThreads), 0, st, j));
   return 0;
 }
 
