@@ -294,35 +294,27 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
         }
     }
     if (p.q != nullptr) {
-      uint32_t m = 0;
+      float amax = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (tid + i * tpr < chunks) {
-#pragma unroll
-          for (int j = 0; j < N2; ++j) {
-            const float2 v = split(h[i][j]);
-            m = max(m, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
-          }
-        }
-      m = red.max_u32(m);
+        if (tid + i * tpr < chunks) amax = max_abs_nan(amax, h[i]);
+      const uint32_t m = red.max_u32(__float_as_uint(amax) & 0x7fffffffu);
       const float sc = int8_scale(m);
       const bool bad = m >= 0x7f800000u;
       const float inv = __frcp_rn(sc);
       if (tid == 0) p.q_scale[t] = sc;
+      uint8_t* qo = reinterpret_cast<uint8_t*>(p.q + t * p.H) + tid * VEC;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = tid + i * tpr;
-        if (c < chunks) {
-          Pack<int8_t, VEC> k;
-#pragma unroll
-          for (int j = 0; j < N2; ++j) {
-            const float2 v = split(h[i][j]);
-            k.v[2 * j] = bad ? (int8_t)0 : (int8_t)quant_int8(v.x, sc, inv);
-            k.v[2 * j + 1] = bad ? (int8_t)0 : (int8_t)quant_int8(v.y, sc, inv);
+      for (int i = 0; i < NV; ++i)
+        if (tid + i * tpr < chunks) {
+          uint32_t k[N2 / 2];
+          quant_int8(h[i], sc, inv, k);
+          if constexpr (N2 == 4) {
+            *reinterpret_cast<uint2*>(qo + i * tpr * VEC) = bad ? make_uint2(0, 0) : make_uint2(k[0], k[1]);
+          } else {
+            *reinterpret_cast<uint32_t*>(qo + i * tpr * VEC) = bad ? 0u : k[0];
           }
-          *reinterpret_cast<Pack<int8_t, VEC>*>(p.q + t * p.H + c * VEC) = k;
         }
-      }
     }
     const uint32_t swap = at;
     at = other;

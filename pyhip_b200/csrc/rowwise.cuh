@@ -295,4 +295,53 @@ __device__ __forceinline__ int quant_int8(float v, float s, float inv) {
   return off ? qi + (d > 0.f ? 1 : -1) : qi;
 }
 
+// max(|a|, |b|) in magnitude (the sign means nothing), NaN if either is
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+  float d;
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+template <int N2>
+__device__ __forceinline__ float max_abs_nan(float m, const f32x2 (&v)[N2]) {
+#pragma unroll
+  for (int j = 0; j < N2; ++j) {
+    const float2 x = split(v[j]);
+    m = max_abs_nan(max_abs_nan(m, x.x), x.y);
+  }
+  return m;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 2 N2 values to 8-bit integers, four to a word.  v * inv + 1.5 * 2^23 holds the nearest whole number in its low bits (the
+// conversions between float and integer run at an eighth of the rate); where a remainder reaches s/2 the exact rule above
+// decides again, which is rare.
+template <int N2>
+__device__ __forceinline__ void quant_int8(const f32x2 (&v)[N2], float s, float inv, uint32_t (&out)[N2 / 2]) {
+  const f32x2 inv2 = both(inv), magic = both(12582912.f), minus = both(-12582912.f), ms = both(-s);
+  uint32_t b[2 * N2];
+  float worst = 0.f;
+#pragma unroll
+  for (int j = 0; j < N2; ++j) {
+    const f32x2 m = fma2(v[j], inv2, magic);
+    const float2 k = split(m), d = split(fma2(add2(m, minus), ms, v[j]));
+    b[2 * j] = __float_as_uint(k.x);
+    b[2 * j + 1] = __float_as_uint(k.y);
+    worst = fmaxf(fmaxf(worst, fabsf(d.x)), fabsf(d.y));
+  }
+  if (worst >= 0.5f * s) {
+#pragma unroll
+    for (int j = 0; j < N2; ++j) {
+      const float2 x = split(v[j]);
+      b[2 * j] = (uint32_t)quant_int8(x.x, s, inv);
+      b[2 * j + 1] = (uint32_t)quant_int8(x.y, s, inv);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < N2 / 2; ++j)
+    out[j] = __byte_perm(__byte_perm(b[4 * j], b[4 * j + 1], 0x0040), __byte_perm(b[4 * j + 2], b[4 * j + 3], 0x0040), 0x5410);
+}
+
 }  // namespace b200moe
