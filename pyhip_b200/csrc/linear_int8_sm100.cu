@@ -5,7 +5,9 @@
 // Two kernels, chosen by size (pick_variant):
 //   split   one 128-feature x BT-token tile per CTA, the weights on the MMA's M side; the CTAs of a cluster take equal
 //           ranges of K and add their tiles through distributed shared memory.  For few tokens, where the weights' bytes
-//           and the launch latency bound the call: every weight byte is requested as soon as the CTA starts.
+//           and the launch latency bound the call: every weight byte is requested as soon as the CTA starts.  A handful of
+//           tokens are quantised here too, by the epilogue warps while the weights are on their way: every CTA reads the
+//           rows for their scales and converts its own range of K (one launch instead of two, and no workspace).
 //   pair    persistent CTA pairs (cta_group::2), 256 tokens x BN features a tile: each CTA holds its 128 tokens' rows and
 //           half of the feature rows, two accumulators overlap a tile's epilogue with the next one's products.
 //
@@ -42,7 +44,9 @@ struct LinearParams {
   const float* bias;
   void* y;
   int32_t* status;
-  int T, N, KB, k_tail_steps, stages, fp16, store_tma, early_weights;
+  const void* x;        // rows that the split kernel quantises itself
+  int64_t x_stride;
+  int T, N, K, KB, k_tail_steps, stages, fp16, store_tma, early_weights, x_dtype, x_vec;
   int tokens, splits;             // split: token tile, CTAs that share K
   int m_tiles, n_tiles;           // pair
 };
@@ -139,14 +143,79 @@ __device__ __forceinline__ void drain_copies(SmemCtlI8* ctl, int64_t issued, int
 }
 
 // ------------------------------------------------------------------------------------ split
+constexpr int kFusedTokens = 8;                 // rows that the split kernel quantises itself, at most
+constexpr int kFusedTile = 16;                  // token tile of the MMA then
+constexpr int kFusedBlockBytes = kFusedTile * kTileKI8;
+constexpr int kFusedBlocks = 16;                // k-blocks of a CTA, at most
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// 16 neighbouring values of a row as pairs
+template <typename T>
+__device__ __forceinline__ void load_16(const T* src, bool vec, f32x2 (&v)[8]) {
+  if (vec) {
+    constexpr int P = kPairs<T>;
+#pragma unroll
+    for (int i = 0; i < 8 / P; ++i) {
+      f32x2 part[P];
+      unpack16(reinterpret_cast<const uint4*>(src)[i], part, T());
+#pragma unroll
+      for (int j = 0; j < P; ++j) v[i * P + j] = part[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = pair(to_f(src[2 * i]), to_f(src[2 * i + 1]));
+  }
+}
+// The epilogue warps' part of the fused split kernel: scales of all rows, then this CTA's k-blocks of them as the MMA's N-side
+// tiles (16 rows of 128 bytes in the 128-byte swizzle; rows beyond T are zero).
+template <typename T>
+__device__ __forceinline__ void quantise_rows(const LinearParams& p, uint32_t tiles, int kb0, int blocks, uint32_t* maxima, float* scales) {
+  const int te = (int)threadIdx.x - 64, warp = te >> 5;
+  const T* x = static_cast<const T*>(p.x);
+  const bool vec = p.x_vec != 0;
+  const int pieces = p.K / 16;
+  for (int t = 0; t < p.T; ++t) {
+    float m = 0.f;
+#pragma unroll 2
+    for (int c = te; c < pieces; c += 128) {
+      f32x2 v[8];
+      load_16<T>(x + t * p.x_stride + c * 16, vec, v);
+      m = max_abs_nan(m, v);
+    }
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7fffffffu);
+    if ((te & 31) == 0) maxima[t * 4 + warp] = bits;
+  }
+  epilogue_sync();
+  if (te < p.T) scales[te] = int8_scale(max(max(maxima[te * 4], maxima[te * 4 + 1]), max(maxima[te * 4 + 2], maxima[te * 4 + 3])));
+  epilogue_sync();
+  const int per_row = blocks * 8;                          // 16-byte pieces of a row in this CTA's range
+  for (int i = te; i < kFusedTile * per_row; i += 128) {
+    const int t = i / per_row, c = i - t * per_row, k = kb0 * kTileKI8 + c * 16;
+    uint32_t o[4] = {0, 0, 0, 0};
+    if (t < p.T && k < p.K) {
+      const float s = scales[t];
+      if (s == s) {                                        // (a row with an infinity or NaN: zeros, and scale NaN)
+        f32x2 v[8];
+        load_16<T>(x + t * p.x_stride + k, vec, v);
+        quant_int8(v, s, __frcp_rn(s), o);
+      }
+    }
+    st_shared_v4(tiles + (uint32_t)(c >> 3) * kFusedBlockBytes + (uint32_t)t * kTileKI8 + (uint32_t)(((c & 7) ^ (t & 7)) << 4), o[0], o[1], o[2], o[3]);
+  }
+}
+
+template <bool FUSED>
 __global__ void __launch_bounds__(kThreadsI8)
 linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
   extern __shared__ uint8_t smem_raw[];
+  __shared__ uint32_t maxima[FUSED ? kFusedTokens * 4 : 1];
+  __shared__ float scales[FUSED ? kFusedTokens : 1];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   SmemCtlI8* ctl = reinterpret_cast<SmemCtlI8*>(smem);
   const uint32_t stage0 = smem_u32(smem) + kCtlBytes;
   const int S = p.stages, BT = p.tokens, C = p.splits;
-  const uint32_t stage_bytes = (uint32_t)(kRowTileBytes + BT * kTileKI8);
+  const uint32_t stage_bytes = (uint32_t)(kRowTileBytes + (FUSED ? 0 : BT * kTileKI8));
+  const uint32_t token_tiles = stage0 + S * stage_bytes;   // FUSED: one for each k-block of the CTA
   const uint32_t cols = (uint32_t)max(32, BT);             // BT is 16 or a power of two from 32 to 256
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)(blockIdx.x % (unsigned)C);        // clusters run along x
@@ -160,6 +229,7 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
       mbar_init(smem_u32(&ctl->empty[s]), 1);
     }
     mbar_init(smem_u32(&ctl->tmem_full[0]), 1);
+    mbar_init(smem_u32(&ctl->tmem_empty[0]), 1);           // FUSED: the token tiles are ready
     ctl->abort_word = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -179,7 +249,7 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
       // The weights do not depend on the launch in front when that is this call's own quantiser (early_weights): it
       // lets this grid start only after everything before it has completed.
       int ahead = 0;
-      if (p.early_weights)
+      if (!FUSED && p.early_weights)
         for (; ahead < min(S, kb1 - kb0); ++ahead) {
           const uint32_t full = smem_u32(&ctl->full[ahead]);
           mbar_expect_tx(full, stage_bytes);
@@ -196,7 +266,7 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
           mbar_expect_tx(full, stage_bytes);
           tma_load_2d(st, &p.tmW, full, kb * kTileKI8, n0);
         }
-        tma_load_2d(st + kRowTileBytes, &p.tmX, full, kb * kTileKI8, t0);
+        if (!FUSED) tma_load_2d(st + kRowTileBytes, &p.tmX, full, kb * kTileKI8, t0);
         ++issued;
         if (++stage == S) { stage = 0; phase ^= 1; }
       }
@@ -206,13 +276,14 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
     const uint32_t idesc = make_idesc_i8(kRowTile, (uint32_t)BT);
     int stage = 0;
     uint32_t phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
+    if (FUSED) ok = mbar_wait(smem_u32(&ctl->tmem_empty[0]), 0, abort_word, 0x1400);
+    for (int kb = kb0; kb < kb1 && ok; ++kb) {
       if (!mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_word, 0x1200 + stage)) { ok = false; break; }
       tc_fence_after_sync();
       __syncwarp();
       if (elect_one()) {
         const uint32_t st = stage0 + stage * stage_bytes;
-        const uint32_t a_lo = desc_lo_sw(st), b_lo = desc_lo_sw(st + kRowTileBytes);
+        const uint32_t a_lo = desc_lo_sw(st), b_lo = desc_lo_sw(FUSED ? token_tiles + (uint32_t)(kb - kb0) * kFusedBlockBytes : st + kRowTileBytes);
         const int steps = kb == p.KB - 1 ? p.k_tail_steps : 4;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
@@ -226,6 +297,14 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
     grid_dep_wait();
   } else {
     grid_dep_wait();
+    if (FUSED) {
+      if (p.x_dtype == B200MOE_T_BF16) quantise_rows<__nv_bfloat16>(p, token_tiles, kb0, kb1 - kb0, maxima, scales);
+      else if (p.x_dtype == B200MOE_T_FP16) quantise_rows<__half>(p, token_tiles, kb0, kb1 - kb0, maxima, scales);
+      else quantise_rows<float>(p, token_tiles, kb0, kb1 - kb0, maxima, scales);
+      fence_proxy_async_smem();
+      epilogue_sync();
+      if (threadIdx.x == 64) mbar_arrive(smem_u32(&ctl->tmem_empty[0]));
+    }
   }
   grid_dep_launch();
 
@@ -266,7 +345,7 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
       const int4 v = ld_peer_v4(peer_smem(at, (uint32_t)r));
       a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
     }
-    const float xs = p.x_scale[t0 + c];
+    const float xs = FUSED ? scales[c] : p.x_scale[t0 + c];
     const float o0 = fmaf((float)a.x * xs, ws[0], bs[0]), o1 = fmaf((float)a.y * xs, ws[1], bs[1]);
     const float o2 = fmaf((float)a.z * xs, ws[2], bs[2]), o3 = fmaf((float)a.w * xs, ws[3], bs[3]);
     const uint32_t lo = pack2(o0, o1, p.fp16), hi = pack2(o2, o3, p.fp16);
@@ -493,12 +572,13 @@ int encode_rows(CUtensorMap* map, const void* base, int K, int rows, int box_row
 }
 
 struct Variant {
-  bool pair;
+  bool pair, fused;
   int tokens, splits, stages;    // split
   int bn;                        // pair
 };
 
-Variant pick_variant(int T, int N, int KB, int force) {
+Variant pick_variant(int T, int N, int K, int force, bool quantise) {
+  const int KB = (K + kTileKI8 - 1) / kTileKI8;
   Variant v = {};
   const int sms = device_sm_count();
   v.pair = force == 2 || (force == 0 && T > 256);
@@ -511,50 +591,65 @@ Variant pick_variant(int T, int N, int KB, int force) {
   const int64_t tiles = (int64_t)((N + kRowTile - 1) / kRowTile) * ((T + v.tokens - 1) / v.tokens);
   v.splits = 1;
   while (v.splits < 8 && tiles * v.splits * 2 <= 3 * sms && KB / (v.splits * 2) >= 2) v.splits *= 2;
-  const int stage = kRowTileBytes + v.tokens * kTileKI8;
   const int kb = (KB + v.splits - 1) / v.splits;
+  // Every CTA reads all rows: 64 KB at most, against the 16 KB of weights of each of its k-blocks.
+  v.fused = quantise && T <= kFusedTokens && (int64_t)T * KB * kTileKI8 <= 32768 && kb <= kFusedBlocks;
+  const int stage = kRowTileBytes + (v.fused ? 0 : v.tokens * kTileKI8);
   v.stages = std::min({kb, kMaxStagesI8, 110 * 1024 / stage});
   return v;
 }
 
 }  // namespace
 
-int launch_linear_int8(const void* q, const float* x_scale, const void* w, const float* w_scale, const float* bias, void* y, int T,
-                       int N, int K, int fp16, int early_weights, int variant, int32_t* status, cudaStream_t st) {
+struct LinearArgs {
+  const void* x; int64_t x_stride; int x_dtype;        // rows; int8 ones with q = x and their scale
+  const void* q; const float* x_scale;
+  const void* w; const float* w_scale; const float* bias;
+  void* y;
+  int T, N, K, fp16, early_weights;
+  int32_t* status;
+};
+int launch_linear_int8(const LinearArgs& a, const Variant& v, cudaStream_t st) {
   LinearParams p;
   memset(&p, 0, sizeof(p));
+  const int T = a.T, N = a.N, K = a.K;
+  p.K = K;
   p.KB = (K + kTileKI8 - 1) / kTileKI8;
   p.k_tail_steps = (K - (p.KB - 1) * kTileKI8 + 31) / 32;
-  p.T = T; p.N = N; p.x_scale = x_scale; p.w_scale = w_scale; p.bias = bias; p.y = y; p.status = status; p.fp16 = fp16;
-  const Variant v = pick_variant(T, N, p.KB, variant);
+  p.T = T; p.N = N; p.x_scale = a.x_scale; p.w_scale = a.w_scale; p.bias = a.bias; p.y = a.y; p.status = a.status; p.fp16 = a.fp16;
   if (!v.pair) {
-    p.tokens = v.tokens; p.splits = v.splits; p.stages = v.stages; p.early_weights = early_weights;
-    if (int rc = encode_rows(&p.tmX, q, K, T, v.tokens, "int8 token rows")) return rc;
-    if (int rc = encode_rows(&p.tmW, w, K, N, kRowTile, "int8 weights")) return rc;
+    p.tokens = v.tokens; p.splits = v.splits; p.stages = v.stages; p.early_weights = a.early_weights;
+    p.x = a.x; p.x_stride = a.x_stride; p.x_dtype = a.x_dtype;
+    const int64_t row = 16 / (a.x_dtype == B200MOE_T_FP32 ? 4 : 2);
+    p.x_vec = ((uintptr_t)a.x & 15) == 0 && a.x_stride % row == 0;
+    if (!v.fused)
+      if (int rc = encode_rows(&p.tmX, a.q, K, T, v.tokens, "int8 token rows")) return rc;
+    if (int rc = encode_rows(&p.tmW, a.w, K, N, kRowTile, "int8 weights")) return rc;
     const int n_tiles = (N + kRowTile - 1) / kRowTile, t_tiles = (T + v.tokens - 1) / v.tokens;
     B200_CHECK_ARG(t_tiles <= 65535, "linear_int8: %d tokens", T);
-    const int stage = kRowTileBytes + v.tokens * kTileKI8;
+    const int stage = kRowTileBytes + (v.fused ? 0 : v.tokens * kTileKI8);
+    const int blocks = v.fused ? ((p.KB + v.splits - 1) / v.splits) * kFusedBlockBytes : 0;
     // At least the share of shared memory that its columns are of tensor memory: CTAs that fit an SM's shared memory
     // then fit its tensor memory too, and no cluster waits for columns that another waiting cluster holds.
     const int share = (int)((int64_t)kSmemLimitI8 * std::max(32, v.tokens) / 512);
-    const int bytes = std::max({v.stages * stage, std::min(v.tokens, T) * kRowTile * 4 + 16 * kRowTile * 4, share});
+    const int bytes = std::max({v.stages * stage + blocks, std::min(v.tokens, T) * kRowTile * 4 + 16 * kRowTile * 4, share});
     const size_t smem = 1024 + kCtlBytes + (size_t)bytes;
-    B200_CHECK_CUDA(cudaFuncSetAttribute(linear_int8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimitI8));
-    B200_CHECK_CUDA(launch_chained_cluster(linear_int8_split_kernel, dim3(n_tiles * v.splits, t_tiles), dim3(kThreadsI8), smem, st,
-                                           v.splits, p));
+    void (*k)(LinearParams) = v.fused ? linear_int8_split_kernel<true> : linear_int8_split_kernel<false>;
+    B200_CHECK_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimitI8 - 1024));
+    B200_CHECK_CUDA(launch_chained_cluster(k, dim3(n_tiles * v.splits, t_tiles), dim3(kThreadsI8), smem, st, v.splits, p));
     return 0;
   }
   const int bn = v.bn;
   p.m_tiles = (T + 255) / 256;
   p.n_tiles = (N + bn - 1) / bn;
-  if (int rc = encode_rows(&p.tmX, q, K, T, 128, "int8 token rows")) return rc;
-  if (int rc = encode_rows(&p.tmW, w, K, N, bn / 2, "int8 weights")) return rc;
-  p.store_tma = N % 8 == 0 && ((uintptr_t)y & 15) == 0;
+  if (int rc = encode_rows(&p.tmX, a.q, K, T, 128, "int8 token rows")) return rc;
+  if (int rc = encode_rows(&p.tmW, a.w, K, N, bn / 2, "int8 weights")) return rc;
+  p.store_tma = N % 8 == 0 && ((uintptr_t)a.y & 15) == 0;
   if (p.store_tma) {
     cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)T};
     cuuint64_t strides[1] = {(cuuint64_t)N * 2};
     cuuint32_t box[2] = {kStoreCols, 32};
-    if (int rc = encode_map_sw(&p.tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+    if (int rc = encode_map_sw(&p.tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
                                CU_TENSOR_MAP_L2_PROMOTION_NONE, "linear output"))
       return rc;
   }
@@ -576,7 +671,8 @@ using namespace b200moe;
 
 extern "C" int b200moe_linear_int8_workspace(int32_t T, int32_t N, int32_t K, int32_t variant, int64_t* bytes) {
   B200_CHECK_ARG(bytes != nullptr && T >= 0 && N >= 1 && K >= 1 && variant >= 0 && variant <= 2, "linear_int8_workspace: T=%d N=%d K=%d", T, N, K);
-  *bytes = T == 0 ? 0 : round_up64((int64_t)T * K, 256) + (int64_t)T * 4;     // the quantised rows and their scales
+  const Variant v = pick_variant(T, N, K, variant, true);
+  *bytes = T == 0 || v.fused ? 0 : round_up64((int64_t)T * K, 256) + (int64_t)T * 4;     // the quantised rows and their scales
   return 0;
 }
 
@@ -593,19 +689,22 @@ extern "C" int b200moe_linear_int8(const void* x, int64_t x_stride, int32_t x_dt
   B200_CHECK_ARG(((uintptr_t)weight & 15) == 0, "linear_int8: weight must be 16-byte aligned");
   B200_CHECK_ARG(((uintptr_t)y & 7) == 0, "linear_int8: y must be 8-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;
-  const void* q = x;
-  const float* scale = x_scale;
-  if (x_dtype != B200MOE_T_INT8) {
-    // the quantised rows and their scales
-    const int64_t rows = round_up64((int64_t)T * K, 256);
-    B200_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= rows + (int64_t)T * 4,
-                   "linear_int8: workspace holds %lld bytes of %lld", (long long)workspace_bytes, (long long)(rows + (int64_t)T * 4));
-    q = workspace;
-    scale = (const float*)((uint8_t*)workspace + rows);
-    if (int rc = b200moe_quantize_int8(x, x_stride, T, K, x_dtype, workspace, const_cast<float*>(scale), stream)) return rc;
-  } else {
+  const bool quantise = x_dtype != B200MOE_T_INT8;
+  const Variant v = pick_variant(T, N, K, variant, quantise);
+  LinearArgs a = {x, x_stride, x_dtype, x, x_scale, weight, weight_scale, bias, y, T, N, K, out_dtype == B200MOE_T_FP16, quantise, status};
+  if (!quantise) {
     B200_CHECK_ARG(x_scale != nullptr && x_stride == K && ((uintptr_t)x & 15) == 0, "linear_int8: 8-bit rows must be contiguous, 16-byte aligned and have x_scale");
+  } else {
+    B200_CHECK_ARG(K <= 16384 && x_stride >= 0, "linear_int8: rows of %d values, %lld apart", K, (long long)x_stride);
+    if (!v.fused) {
+      const int64_t rows = round_up64((int64_t)T * K, 256);
+      B200_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= rows + (int64_t)T * 4,
+                     "linear_int8: workspace holds %lld bytes of %lld", (long long)workspace_bytes, (long long)(rows + (int64_t)T * 4));
+      float* scale = (float*)((uint8_t*)workspace + rows);
+      if (int rc = b200moe_quantize_int8(x, x_stride, T, K, x_dtype, workspace, scale, stream)) return rc;
+      a.q = workspace;
+      a.x_scale = scale;
+    }
   }
-  return launch_linear_int8(q, scale, weight, weight_scale, bias, y, T, N, K, out_dtype == B200MOE_T_FP16, x_dtype != B200MOE_T_INT8, variant,
-                            status, st);
+  return launch_linear_int8(a, v, st);
 }

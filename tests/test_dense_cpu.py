@@ -17,7 +17,7 @@ def L():
     return _lib.lib()
 
 
-def _linear(L, x=P, stride=64, dt=_lib.T_BF16, xs=None, w=P, ws=P, bias=None, T=4, N=32, K=64, out=_lib.T_BF16, variant=0, work=P, size=1 << 20, y=P):
+def _linear(L, x=P, stride=64, dt=_lib.T_BF16, xs=None, w=P, ws=P, bias=None, T=40, N=32, K=64, out=_lib.T_BF16, variant=0, work=P, size=1 << 20, y=P):
     return L.b200moe_linear_int8(x, stride, dt, xs, w, ws, bias, T, N, K, out, variant, work, size, None, y, None)
 
 

@@ -94,6 +94,22 @@ def test_layer_matches_64_bits(T, N, K, variant):
     assert int8_status(DEV) == (0, 0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,N,K", [(1, 2880, 2880), (1, 129, 16384), (8, 300, 4096), (3, 2880, 2896), (5, 14336, 2048), (8, 64, 16), (9, 64, 4096), (2, 40, 8208)])
+def test_few_tokens(T, N, K, dtype):
+    """The sizes around those that the split kernel quantises itself: rows on and off the 16-byte grid, apart from one another,
+    the last ones of a buffer."""
+    g = torch.Generator().manual_seed(T * K)
+    w, ws = _weight(N, K, T)
+    wide = torch.randn(T, K + 24, generator=g).to(dtype).to(DEV)
+    for x in (wide[:, :K].contiguous(), wide[:, 8:K + 8], wide[:, 3:K + 3], wide[:, 24:]):
+        y = linear_int8(x, w, ws, out_dtype=torch.bfloat16)
+        _check(y, *orc.linear_int8(*orc.quantize_int8(x), w, ws))
+        q, s = quantize_int8(x)
+        assert torch.equal(y, linear_int8(q, w, ws, x_scale=s, out_dtype=torch.bfloat16))
+    assert int8_status(DEV) == (0, 0)
+
+
 @pytest.mark.parametrize("T,N,K", [(4, 64, 16), (600, 264, 1040), (2000, 1160, 512), (5000, 515, 256)])
 def test_layer_types_bias_and_prequantised_rows(T, N, K):
     g = torch.Generator().manual_seed(T)
