@@ -119,6 +119,14 @@ __device__ __forceinline__ int4 ld_peer_v4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ void st_peer_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
@@ -380,11 +388,20 @@ __device__ __forceinline__ void tile_of(int w, int m_tiles, int n_tiles, int& m,
   n = in / height;
 }
 
-template <int BN>
+// arrive on the barrier at this offset in both CTAs of pair `z` of the cluster once the products issued so far are done
+__device__ __forceinline__ void commit_to_pair(uint32_t bar, uint32_t z) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"((unsigned short)(3u << (2 * z)))
+               : "memory");
+}
+
+// Z pairs of a cluster share one tile's K (Z = 1: persistent, a cluster walks over tiles).  With Z > 1 each pair ends up with
+// BN / Z columns of the tile: the others' partial sums of them arrive in its stages' memory, one slot for each.
+template <int BN, int Z>
 __global__ void __launch_bounds__(kThreadsI8, 1)
 linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
   constexpr uint32_t B_BYTES = BN / 2 * kTileKI8, STAGE = kRowTileBytes + B_BYTES;
-  constexpr uint32_t COLS = 2 * BN;
+  constexpr uint32_t COLS = (Z == 1 ? 2 : 1) * BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   SmemCtlI8* ctl = reinterpret_cast<SmemCtlI8*>(smem);
@@ -393,7 +410,7 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
   const uint32_t staging = stage0 + S * STAGE;                                    // 4 KB for each epilogue warp
   float* scales = reinterpret_cast<float*>(smem + kCtlBytes + S * STAGE + 4 * 4096);   // [2][2][BN]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_cta_rank();
+  const uint32_t rank = cluster_cta_rank() & 1, z = cluster_cta_rank() >> 1;
   volatile uint32_t* abort_word = &ctl->abort_word;
 
   if (threadIdx.x == 0) {
@@ -421,7 +438,8 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
   grid_dep_wait();
   grid_dep_launch();
 
-  const int total = p.m_tiles * p.n_tiles, first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
+  const int total = p.m_tiles * p.n_tiles, first = (int)blockIdx.x / (2 * Z), step = (int)gridDim.x / (2 * Z);
+  const int kb0 = Z == 1 ? 0 : (int)((int64_t)p.KB * z / Z), kb1 = Z == 1 ? p.KB : (int)((int64_t)p.KB * (z + 1) / Z);
   if (warp == 0) {
     if (lane == 0) {
       prefetch_tensormap(&p.tmX);
@@ -434,7 +452,7 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
         int m, n;
         tile_of(w, p.m_tiles, p.n_tiles, m, n);
         const int t0 = m * 256 + (int)rank * 128, n0 = n * BN + (int)rank * (BN / 2);
-        for (int kb = 0; kb < p.KB; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(smem_u32(&ctl->empty[stage]), phase ^ 1, abort_word, 0x2100 + stage)) { ok = false; break; }
           const uint32_t st = stage0 + stage * STAGE, full = smem_u32(&ctl->full[stage]);
           if (rank == 0) mbar_expect_tx(full, 2 * STAGE);
@@ -454,7 +472,7 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
     for (int w = rank == 0 ? first : total; w < total && ok; w += step) {
       if (!mbar_wait(smem_u32(&ctl->tmem_empty[acc]), acc_phase ^ 1, abort_word, 0x2200 + acc)) break;
       tc_fence_after_sync();
-      for (int kb = 0; kb < p.KB; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(smem_u32(&ctl->full[stage]), phase, abort_word, 0x2300 + stage)) { ok = false; break; }
         tc_fence_after_sync();
         __syncwarp();
@@ -464,9 +482,9 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
           const int steps = kb == p.KB - 1 ? p.k_tail_steps : 4;
 #pragma unroll
           for (int s = 0; s < 4; ++s)
-            if (s < steps) umma_i8<true>(tmem_base + acc * BN, a_lo + 2 * s, b_lo + 2 * s, idesc, (kb != 0 || s != 0) ? 1u : 0u);
-          tc_commit_pair(smem_u32(&ctl->empty[stage]));
-          if (kb == p.KB - 1) tc_commit_pair(smem_u32(&ctl->tmem_full[acc]));
+            if (s < steps) umma_i8<true>(tmem_base + acc * BN, a_lo + 2 * s, b_lo + 2 * s, idesc, (kb != kb0 || s != 0) ? 1u : 0u);
+          commit_to_pair(smem_u32(&ctl->empty[stage]), z);
+          if (kb == kb1 - 1) commit_to_pair(smem_u32(&ctl->tmem_full[acc]), z);
         }
         __syncwarp();
         if (++stage == S) { stage = 0; phase ^= 1; }
@@ -474,8 +492,35 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
-  } else {
-    const int quad = warp & 3, te = threadIdx.x - 64;
+  }
+  const int quad = warp & 3, te = (int)threadIdx.x - 64;
+  const uint32_t rows_at = stage0 + (uint32_t)(quad * 32 + lane) * 4;     // Z > 1: [slot][column][128 rows] int32
+  bool ready = false;
+  if constexpr (Z > 1) {
+    // every product of the cluster is done before anything is written over its operands
+    if (warp >= 2) ready = mbar_wait(smem_u32(&ctl->tmem_full[0]), 0, abort_word, 0x2400);
+    __syncwarp();
+    tc_fence_before_sync();
+    cluster_sync_all();
+    tc_fence_after_sync();
+    if (warp >= 2 && ready) {
+      for (int d = 1; d < Z; ++d) {
+        const uint32_t to = (z + d) % Z, slot = Z - 1 - d;               // the receiver counts its senders from behind
+        const uint32_t dst = peer_smem(rows_at, 2 * to + rank) + slot * (BN / Z) * 512;
+#pragma unroll 1
+        for (int c = 0; c < BN / Z; c += 16) {
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(tmem_base + ((uint32_t)(quad * 32) << 16) + to * (BN / Z) + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) st_peer_u32(dst + (uint32_t)(c + i) * 512, v[i]);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+  }
+  if (warp >= 2) {
     const uint32_t mine = staging + (uint32_t)(warp - 2) * 4096;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -490,15 +535,16 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
         sc[BN + i] = (in && p.bias != nullptr) ? p.bias[n0 + i] : 0.f;
       }
       const float xs = row0 + lane < p.T ? p.x_scale[row0 + lane] : 0.f;
-      const bool ok = mbar_wait(smem_u32(&ctl->tmem_full[acc]), acc_phase, abort_word, 0x2400 + acc);
+      const bool ok = Z > 1 ? ready : mbar_wait(smem_u32(&ctl->tmem_full[acc]), acc_phase, abort_word, 0x2400 + acc);
       uint32_t all;                        // every epilogue warp of the CTA sees the scales, or all of them give up
       asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                    : "=r"(all) : "r"((uint32_t)ok) : "memory");
       if (!all) break;
       tc_fence_after_sync();
       const uint32_t tacc = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN;
+      const int first_col = Z > 1 ? (int)z * (BN / Z) : 0;
 #pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += kStoreCols) {
+      for (int c0 = first_col; c0 < first_col + BN / Z; c0 += kStoreCols) {
         if (row0 >= p.T || n0 + c0 >= p.N) break;
         if (lane == 0) bulk_wait_read();    // the staging rows' previous copy has been read out
         __syncwarp();
@@ -507,6 +553,12 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
           uint32_t v[16];
           tmem_ld_32x32b_x16(tacc + c0 + h, v);
           tmem_ld_wait();
+          if constexpr (Z > 1) {
+#pragma unroll
+            for (int slot = 0; slot < Z - 1; ++slot)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] += ld_shared_u32(rows_at + (uint32_t)(slot * (BN / Z) + c0 - first_col + h + i) * 512);
+          }
           uint32_t o[8];
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
@@ -533,7 +585,7 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
           const int col = n0 + c0 + lane * 2;
           for (int r = 0; r < 32 && row0 + r < p.T; ++r) {
             uint32_t v;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(mine + (uint32_t)r * 128 + ((((uint32_t)lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4));
+            v = ld_shared_u32(mine + (uint32_t)r * 128 + ((((uint32_t)lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
             uint16_t* dst = static_cast<uint16_t*>(p.y) + (int64_t)(row0 + r) * p.N + col;
             if (col < p.N) dst[0] = (uint16_t)v;
             if (col + 1 < p.N) dst[1] = (uint16_t)(v >> 16);
@@ -574,7 +626,7 @@ int encode_rows(CUtensorMap* map, const void* base, int K, int rows, int box_row
 struct Variant {
   bool pair, fused;
   int tokens, splits, stages;    // split
-  int bn;                        // pair
+  int bn, z;                     // pair: features of a tile, pairs that share K
 };
 
 Variant pick_variant(int T, int N, int K, int force, bool quantise) {
@@ -583,8 +635,19 @@ Variant pick_variant(int T, int N, int K, int force, bool quantise) {
   const int sms = device_sm_count();
   v.pair = force == 2 || (force == 0 && T > 256);
   if (v.pair) {
-    const int64_t tiles = (int64_t)((T + 255) / 256) * ((N + 255) / 256);
-    v.bn = tiles * 2 >= sms ? 256 : 128;
+    // Cost of a tile shape: rounds of tiles over the pairs x k-blocks x what one takes, plus what a round does not overlap.
+    // A k-block of 256 features takes 0.38 us and of 128 features 0.28 (both bound by what an SM draws from L2, 24 and
+    // 32 KB), filling, emptying and joining 4 us, joining two halves of K another 1.5.
+    const int pairs = sms / 2, mt = (T + 255) / 256;
+    double best = 0;
+    for (int bn : {256, 128})
+      for (int z : {1, 2}) {
+        const int64_t tiles = (int64_t)mt * ((N + bn - 1) / bn);
+        if (z > 1 && (tiles * z > pairs || KB < 4 * z)) continue;
+        const double rounds = z > 1 ? 1.0 : (double)((tiles + pairs - 1) / pairs);
+        const double cost = rounds * ((KB + z - 1) / z) * (bn == 256 ? 0.38 : 0.28) + 4.0 + (z > 1 ? 1.5 : 0.0);
+        if (v.bn == 0 || cost < best) { best = cost; v.bn = bn; v.z = z; }
+      }
     return v;
   }
   v.tokens = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
@@ -658,10 +721,11 @@ int launch_linear_int8(const LinearArgs& a, const Variant& v, cudaStream_t st) {
   const size_t smem = 1024 + kCtlBytes + (size_t)p.stages * stage + 4 * 4096 + kPairScaleBytes;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
   B200_CHECK_ARG(tiles < (1ll << 30), "linear_int8: T=%d N=%d", T, N);
-  const int grid = 2 * (int)std::min<int64_t>(device_sm_count() / 2, tiles);
-  void (*k)(LinearParams) = bn == 256 ? linear_int8_pair_kernel<256> : linear_int8_pair_kernel<128>;
+  const int grid = 2 * v.z * (v.z > 1 ? (int)tiles : (int)std::min<int64_t>(device_sm_count() / 2, tiles));
+  void (*k)(LinearParams) = bn == 256 ? (v.z == 2 ? linear_int8_pair_kernel<256, 2> : linear_int8_pair_kernel<256, 1>)
+                                      : (v.z == 2 ? linear_int8_pair_kernel<128, 2> : linear_int8_pair_kernel<128, 1>);
   B200_CHECK_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimitI8));
-  B200_CHECK_CUDA(launch_chained_cluster(k, dim3(grid), dim3(kThreadsI8), smem, st, 2, p));
+  B200_CHECK_CUDA(launch_chained_cluster(k, dim3(grid), dim3(kThreadsI8), smem, st, 2 * v.z, p));
   return 0;
 }
 

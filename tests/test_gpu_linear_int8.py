@@ -84,7 +84,7 @@ def test_quantiser_reads_strided_rows_and_any_shape():
 
 @pytest.mark.parametrize("variant", [1, 2])
 @pytest.mark.parametrize("T,N,K", [(1, 1, 16), (1, 130, 144), (2, 128, 2880), (16, 256, 128), (17, 1001, 1040), (64, 2880, 512),
-                                   (127, 8, 4096), (129, 136, 16), (256, 300, 640), (333, 1001, 1040), (300, 512, 7168)])
+                                   (127, 8, 4096), (129, 136, 16), (256, 300, 640), (333, 1001, 1040), (300, 512, 7168), (1000, 2048, 7168), (700, 1501, 4096), (1000, 2043, 4096), (2049, 2311, 272)])
 def test_layer_matches_64_bits(T, N, K, variant):
     g = torch.Generator().manual_seed(T + N + K)
     w, ws = _weight(N, K, T + N)
