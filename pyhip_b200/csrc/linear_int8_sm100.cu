@@ -32,13 +32,15 @@ constexpr int kRowTileBytes = kRowTile * kTileKI8;
 constexpr int kMaxStagesI8 = 12;
 constexpr int kSmemLimitI8 = 232448;            // 227 KB
 constexpr int kCtlBytes = 1024;
-constexpr int kStoreCols = 64;                  // columns of a staged store: 128 bytes of a 16-bit type
+constexpr int kPairThreads = 320;               // the same with eight epilogue warps, 2-9
+constexpr int kStoreCols = 32;                  // columns of a staged store: 64 bytes of a 16-bit type
+constexpr int kStagingBytes = 32 * 64;          // 32 rows of them
 constexpr int kPairScaleBytes = 2 * 2 * 256 * 4;   // two tiles' channel scales and biases
 
 struct LinearParams {
   CUtensorMap tmX;      // token rows (K, T)
   CUtensorMap tmW;      // weight rows (K, N)
-  CUtensorMap tmY;      // output (N, T), box 64 x 32; only when store_tma
+  CUtensorMap tmY;      // output (N, T), box 32 x 32; only when store_tma
   const float* x_scale;
   const float* w_scale;
   const float* bias;
@@ -119,8 +121,8 @@ __device__ __forceinline__ int4 ld_peer_v4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
-__device__ __forceinline__ void st_peer_u32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+__device__ __forceinline__ void st_peer_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ uint32_t ld_shared_u32(uint32_t addr) {
   uint32_t v;
@@ -398,7 +400,7 @@ __device__ __forceinline__ void commit_to_pair(uint32_t bar, uint32_t z) {
 // Z pairs of a cluster share one tile's K (Z = 1: persistent, a cluster walks over tiles).  With Z > 1 each pair ends up with
 // BN / Z columns of the tile: the others' partial sums of them arrive in its stages' memory, one slot for each.
 template <int BN, int Z>
-__global__ void __launch_bounds__(kThreadsI8, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
 linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
   constexpr uint32_t B_BYTES = BN / 2 * kTileKI8, STAGE = kRowTileBytes + B_BYTES;
   constexpr uint32_t COLS = (Z == 1 ? 2 : 1) * BN;
@@ -407,8 +409,8 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
   SmemCtlI8* ctl = reinterpret_cast<SmemCtlI8*>(smem);
   const int S = p.stages;
   const uint32_t stage0 = smem_u32(smem) + kCtlBytes;
-  const uint32_t staging = stage0 + S * STAGE;                                    // 4 KB for each epilogue warp
-  float* scales = reinterpret_cast<float*>(smem + kCtlBytes + S * STAGE + 4 * 4096);   // [2][2][BN]
+  const uint32_t staging = stage0 + S * STAGE;                                    // kStagingBytes for each epilogue warp
+  float* scales = reinterpret_cast<float*>(smem + kCtlBytes + S * STAGE + 8 * kStagingBytes);   // [2][2][BN]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_cta_rank() & 1, z = cluster_cta_rank() >> 1;
   volatile uint32_t* abort_word = &ctl->abort_word;
@@ -420,7 +422,7 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&ctl->tmem_full[a]), 1);
-      mbar_init(smem_u32(&ctl->tmem_empty[a]), 8);          // the epilogue warps of both CTAs
+      mbar_init(smem_u32(&ctl->tmem_empty[a]), 16);         // the epilogue warps of both CTAs
     }
     ctl->abort_word = 0;
     fence_mbar_init();
@@ -493,12 +495,26 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
       if (acc == 0) acc_phase ^= 1;
     }
   }
-  const int quad = warp & 3, te = (int)threadIdx.x - 64;
-  const uint32_t rows_at = stage0 + (uint32_t)(quad * 32 + lane) * 4;     // Z > 1: [slot][column][128 rows] int32
+  const int quad = warp & 3, half = (warp - 2) >> 2, te = (int)threadIdx.x - 64;
+  const uint32_t rows_at = stage0 + (uint32_t)(quad * 32 + lane) * 16;    // Z > 1: [slot][column / 4][128 rows][4] int32
+  // channel scales and biases of tile columns n0.. into buffer `acc`
+  auto load_scales = [&](int n0, int acc) {
+    float* sc = scales + acc * 2 * BN;
+    for (int i = te; i < BN; i += 256) {
+      const bool in = n0 + i < p.N;
+      sc[i] = in ? p.w_scale[n0 + i] : 0.f;
+      sc[BN + i] = (in && p.bias != nullptr) ? p.bias[n0 + i] : 0.f;
+    }
+  };
   bool ready = false;
   if constexpr (Z > 1) {
     // every product of the cluster is done before anything is written over its operands
-    if (warp >= 2) ready = mbar_wait(smem_u32(&ctl->tmem_full[0]), 0, abort_word, 0x2400);
+    if (warp >= 2) {
+      int m, n;
+      tile_of(first, p.m_tiles, p.n_tiles, m, n);
+      load_scales(n * BN, 0);
+      ready = mbar_wait(smem_u32(&ctl->tmem_full[0]), 0, abort_word, 0x2400);
+    }
     __syncwarp();
     tc_fence_before_sync();
     cluster_sync_all();
@@ -508,12 +524,12 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
         const uint32_t to = (z + d) % Z, slot = Z - 1 - d;               // the receiver counts its senders from behind
         const uint32_t dst = peer_smem(rows_at, 2 * to + rank) + slot * (BN / Z) * 512;
 #pragma unroll 1
-        for (int c = 0; c < BN / Z; c += 16) {
+        for (int c = half * 16; c < BN / Z; c += 32) {
           uint32_t v[16];
           tmem_ld_32x32b_x16(tmem_base + ((uint32_t)(quad * 32) << 16) + to * (BN / Z) + c, v);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) st_peer_u32(dst + (uint32_t)(c + i) * 512, v[i]);
+          for (int i = 0; i < 16; i += 4) st_peer_v4(dst + (uint32_t)(c + i) * 512, v[i], v[i + 1], v[i + 2], v[i + 3]);
         }
       }
     }
@@ -521,30 +537,26 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
     cluster_sync_all();
   }
   if (warp >= 2) {
-    const uint32_t mine = staging + (uint32_t)(warp - 2) * 4096;
+    const uint32_t mine = staging + (uint32_t)(warp - 2) * kStagingBytes;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int w = first; w < total; w += step) {
       int m, n;
       tile_of(w, p.m_tiles, p.n_tiles, m, n);
       const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * BN;
-      float* sc = scales + acc * 2 * BN;
-      for (int i = te; i < BN; i += 128) {
-        const bool in = n0 + i < p.N;
-        sc[i] = in ? p.w_scale[n0 + i] : 0.f;
-        sc[BN + i] = (in && p.bias != nullptr) ? p.bias[n0 + i] : 0.f;
-      }
+      const float* sc = scales + acc * 2 * BN;
+      if (Z == 1) load_scales(n0, acc);
       const float xs = row0 + lane < p.T ? p.x_scale[row0 + lane] : 0.f;
       const bool ok = Z > 1 ? ready : mbar_wait(smem_u32(&ctl->tmem_full[acc]), acc_phase, abort_word, 0x2400 + acc);
       uint32_t all;                        // every epilogue warp of the CTA sees the scales, or all of them give up
-      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                    : "=r"(all) : "r"((uint32_t)ok) : "memory");
       if (!all) break;
       tc_fence_after_sync();
       const uint32_t tacc = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN;
       const int first_col = Z > 1 ? (int)z * (BN / Z) : 0;
 #pragma unroll 1
-      for (int c0 = first_col; c0 < first_col + BN / Z; c0 += kStoreCols) {
+      for (int c0 = first_col + half * kStoreCols; c0 < first_col + BN / Z; c0 += 2 * kStoreCols) {
         if (row0 >= p.T || n0 + c0 >= p.N) break;
         if (lane == 0) bulk_wait_read();    // the staging rows' previous copy has been read out
         __syncwarp();
@@ -557,7 +569,10 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
 #pragma unroll
             for (int slot = 0; slot < Z - 1; ++slot)
 #pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] += ld_shared_u32(rows_at + (uint32_t)(slot * (BN / Z) + c0 - first_col + h + i) * 512);
+              for (int i = 0; i < 16; i += 4) {
+                const uint4 a = lds16(rows_at + (uint32_t)(slot * (BN / Z) + c0 - first_col + h + i) * 512);
+                v[i] += a.x; v[i + 1] += a.y; v[i + 2] += a.z; v[i + 3] += a.w;
+              }
           }
           uint32_t o[8];
 #pragma unroll
@@ -567,10 +582,9 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
             o[i / 2] = pack2(fmaf((float)(int)v[i] * xs, ws.x, bs.x), fmaf((float)(int)v[i + 1] * xs, ws.y, bs.y), p.fp16);
             o[i / 2 + 1] = pack2(fmaf((float)(int)v[i + 2] * xs, ws.z, bs.z), fmaf((float)(int)v[i + 3] * xs, ws.w, bs.w), p.fp16);
           }
-          const uint32_t row = mine + (uint32_t)lane * 128;
-          const uint32_t j = (uint32_t)h / 8;
-          st_shared_v4(row + ((j ^ (lane & 7)) << 4), o[0], o[1], o[2], o[3]);
-          st_shared_v4(row + (((j + 1) ^ (lane & 7)) << 4), o[4], o[5], o[6], o[7]);
+          const uint32_t row = mine + (uint32_t)lane * 64, j = (uint32_t)h / 8, x = ((uint32_t)lane >> 1) & 3;    // 64-byte swizzle
+          st_shared_v4(row + ((j ^ x) << 4), o[0], o[1], o[2], o[3]);
+          st_shared_v4(row + (((j + 1) ^ x) << 4), o[4], o[5], o[6], o[7]);
         }
         if (p.store_tma) {
           fence_proxy_async_smem();
@@ -580,12 +594,11 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
             bulk_commit();
           }
         } else {
-          // rows of y that do not start on 16 bytes: a row at a time, two neighbouring values a lane
+          // rows of y that do not start on 16 bytes: two rows at a time, two neighbouring values a lane
           __syncwarp();
-          const int col = n0 + c0 + lane * 2;
-          for (int r = 0; r < 32 && row0 + r < p.T; ++r) {
-            uint32_t v;
-            v = ld_shared_u32(mine + (uint32_t)r * 128 + ((((uint32_t)lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+          const int col = n0 + c0 + (lane & 15) * 2;
+          for (int r = lane >> 4; r < 32 && row0 + r < p.T; r += 2) {
+            const uint32_t v = ld_shared_u32(mine + (uint32_t)r * 64 + (((((uint32_t)lane & 15) >> 2) ^ (((uint32_t)r >> 1) & 3)) << 4) + (lane & 3) * 4);
             uint16_t* dst = static_cast<uint16_t*>(p.y) + (int64_t)(row0 + r) * p.N + col;
             if (col < p.N) dst[0] = (uint16_t)v;
             if (col + 1 < p.N) dst[1] = (uint16_t)(v >> 16);
@@ -633,11 +646,11 @@ Variant pick_variant(int T, int N, int K, int force, bool quantise) {
   const int KB = (K + kTileKI8 - 1) / kTileKI8;
   Variant v = {};
   const int sms = device_sm_count();
-  v.pair = force == 2 || (force == 0 && T > 256);
+  v.pair = force == 2 || (force == 0 && T > 64);      // T = 64: 9.8 against 10.8 us (4096 x 4096); T = 128: 12.6 against 10.9
   if (v.pair) {
-    // Cost of a tile shape: rounds of tiles over the pairs x k-blocks x what one takes, plus what a round does not overlap.
-    // A k-block of 256 features takes 0.38 us and of 128 features 0.28 (both bound by what an SM draws from L2, 24 and
-    // 32 KB), filling, emptying and joining 4 us, joining two halves of K another 1.5.
+    // Cost of a tile shape in us, fitted to calls of one round (T = 256 to 1000, N = 2048 and 4096, K = 4096 and 7168): rounds
+    // of tiles over the pairs x k-blocks x what one takes, 0.30 for 256 features and 0.216 for 128; what a call does not
+    // overlap, 7.0 and 6.3; joining two halves of K, 2.3 and 1.3.
     const int pairs = sms / 2, mt = (T + 255) / 256;
     double best = 0;
     for (int bn : {256, 128})
@@ -645,7 +658,8 @@ Variant pick_variant(int T, int N, int K, int force, bool quantise) {
         const int64_t tiles = (int64_t)mt * ((N + bn - 1) / bn);
         if (z > 1 && (tiles * z > pairs || KB < 4 * z)) continue;
         const double rounds = z > 1 ? 1.0 : (double)((tiles + pairs - 1) / pairs);
-        const double cost = rounds * ((KB + z - 1) / z) * (bn == 256 ? 0.38 : 0.28) + 4.0 + (z > 1 ? 1.5 : 0.0);
+        const double cost = rounds * ((KB + z - 1) / z) * (bn == 256 ? 0.30 : 0.216) + (bn == 256 ? 7.0 : 6.3) +
+                            (z == 1 ? 0.0 : bn == 256 ? 2.3 : 1.3);
         if (v.bn == 0 || cost < best) { best = cost; v.bn = bn; v.z = z; }
       }
     return v;
@@ -712,20 +726,20 @@ int launch_linear_int8(const LinearArgs& a, const Variant& v, cudaStream_t st) {
     cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)T};
     cuuint64_t strides[1] = {(cuuint64_t)N * 2};
     cuuint32_t box[2] = {kStoreCols, 32};
-    if (int rc = encode_map_sw(&p.tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+    if (int rc = encode_map_sw(&p.tmY, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.y, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B,
                                CU_TENSOR_MAP_L2_PROMOTION_NONE, "linear output"))
       return rc;
   }
   const int stage = kRowTileBytes + bn / 2 * kTileKI8;
-  p.stages = std::min((kSmemLimitI8 - 1024 - kCtlBytes - 4 * 4096 - kPairScaleBytes) / stage, kMaxStagesI8);
-  const size_t smem = 1024 + kCtlBytes + (size_t)p.stages * stage + 4 * 4096 + kPairScaleBytes;
+  p.stages = std::min((kSmemLimitI8 - 1024 - kCtlBytes - 8 * kStagingBytes - kPairScaleBytes) / stage, kMaxStagesI8);
+  const size_t smem = 1024 + kCtlBytes + (size_t)p.stages * stage + 8 * kStagingBytes + kPairScaleBytes;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
   B200_CHECK_ARG(tiles < (1ll << 30), "linear_int8: T=%d N=%d", T, N);
   const int grid = 2 * v.z * (v.z > 1 ? (int)tiles : (int)std::min<int64_t>(device_sm_count() / 2, tiles));
   void (*k)(LinearParams) = bn == 256 ? (v.z == 2 ? linear_int8_pair_kernel<256, 2> : linear_int8_pair_kernel<256, 1>)
                                       : (v.z == 2 ? linear_int8_pair_kernel<128, 2> : linear_int8_pair_kernel<128, 1>);
   B200_CHECK_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimitI8));
-  B200_CHECK_CUDA(launch_chained_cluster(k, dim3(grid), dim3(kThreadsI8), smem, st, 2 * v.z, p));
+  B200_CHECK_CUDA(launch_chained_cluster(k, dim3(grid), dim3(kPairThreads), smem, st, 2 * v.z, p));
   return 0;
 }
 
