@@ -217,12 +217,21 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
         if (next) load_piece<T, P>(p.wn, tid + i * tpr, hold_n[i]);
       }
   }
+  const bool token = GATE == 0 && p.gate_kind == B200MOE_GATE_TOKEN;
+  auto token_gate = [&](int64_t t) {
+    float g[1] = {1.f};
+    if (token && t < p.T) load_param<T, 1>(p.gate, p.gate_f32, t * p.gate_stride, g);
+    return g[0];
+  };
+  float next_gate = token_gate(blockIdx.x);       // a row ahead, as the rows themselves
   uint32_t at = mine, other = mine + stage_bytes;
   for (int64_t t = blockIdx.x; t < p.T; t += step) {
     copy_wait<0>();
     fetch(t + step, other);                       // the stage that the row before has left
     f32x2 h[NV][N2];
     float scale = 1.f;                            // rstd(y) and a token's gate
+    const float gt = next_gate;
+    next_gate = token_gate(t + step);
     if (POST) {
       f32x2 ss = both(0.f);
 #pragma unroll
@@ -236,11 +245,7 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
       scale = rsqrtf(sum * inv_h + p.eps);
       if (tid == 0 && p.rstd != nullptr) p.rstd[t] = scale;
     }
-    if (GATE == 0 && p.gate_kind == B200MOE_GATE_TOKEN) {
-      float g1[1];
-      load_param<T, 1>(p.gate, p.gate_f32, t * p.gate_stride, g1);
-      scale *= g1[0];
-    }
+    if (GATE == 0) scale *= gt;
     const f32x2 scale2 = both(scale), alpha2 = both(p.alpha);
     f32x2 ss = both(0.f);
     uint4* ho = reinterpret_cast<uint4*>(static_cast<T*>(p.h) + t * p.H) + tid;
@@ -442,7 +447,8 @@ block_norm_bwd_kernel(const __grid_constant__ NormBwdParams b) {
 
 // Backward over a ring of rows in shared memory.  What a row needs twice (y, dn) is read from there again instead of held,
 // so that 16 values a thread and their sums over tokens fit the registers.  GATE and P as in the forward kernel.
-template <typename T, typename P, int GATE, bool POST, bool NEXT>
+// HOLD: the weights stay in registers over the rows (a gate's values leave no room for them).
+template <typename T, typename P, int GATE, bool POST, bool NEXT, bool HOLD>
 __global__ void __launch_bounds__(kRowThreads, 1)
 block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
   constexpr int VEC = 16 / sizeof(T), NV = 16 / VEC, N2 = VEC / 2;
@@ -453,7 +459,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
   grid_dep_wait();
   grid_dep_launch();
   const int chunks = p.H / VEC, tpr = (int)blockDim.x, tid = (int)threadIdx.x;
-  const bool res = p.r != nullptr, has_dh = b.dh != nullptr, has_dn = NEXT && b.dn != nullptr;
+  const bool res = NEXT && p.r != nullptr, has_dh = b.dh != nullptr, has_dn = NEXT && b.dn != nullptr;   // (h is needed with NEXT only)
   const uint32_t array_bytes = (uint32_t)chunks * 16;
   const uint32_t at_r = array_bytes, at_h = at_r + (res ? array_bytes : 0), at_n = at_h + (has_dh ? array_bytes : 0);
   const uint32_t at_g = at_n + (has_dn ? array_bytes : 0), stage_bytes = at_g + (GATE == 2 ? array_bytes : 0);
@@ -492,19 +498,50 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
     }
   const int64_t step = gridDim.x;
   fetch(blockIdx.x, mine);
+  // a row's scalars come a row ahead, as the rows themselves: a load in front of the sums would cost every row its latency
+  struct RowScalars {
+    float ry, rh, gt;
+  };
+  auto scalars = [&](int64_t t) {
+    RowScalars r = {1.f, 0.f, 1.f};
+    if (t < p.T) {
+      if (POST) r.ry = p.rstd[t];
+      if (NEXT) r.rh = p.rstd[p.T + t];
+      if (token) {
+        float g[1];
+        load_param<T, 1>(p.gate, p.gate_f32, t * p.gate_stride, g);
+        r.gt = g[0];
+      }
+    }
+    return r;
+  };
+  f32x2 hold_w[HOLD && POST ? NV : 1][N2], hold_n[HOLD && NEXT ? NV : 1][N2];
+  if (HOLD) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + i * tpr < chunks) {
+        if (POST) load_piece<T, P>(p.w, tid + i * tpr, hold_w[i]);
+        if (NEXT) load_piece<T, P>(p.wn, tid + i * tpr, hold_n[i]);
+      }
+  }
+  auto weight_of = [&](int i, f32x2 (&f)[N2]) {
+    if (HOLD) {
+#pragma unroll
+      for (int j = 0; j < N2; ++j) f[j] = hold_w[HOLD && POST ? i : 0][j];
+    } else {
+      load_piece<T, P>(p.w, tid + i * tpr, f);
+    }
+  };
+  RowScalars ahead = scalars(blockIdx.x);
   uint32_t at = mine, other = mine + stage_bytes;
   for (int64_t t = blockIdx.x; t < p.T; t += step) {
     copy_wait<0>();
     fetch(t + step, other);                       // the stage that the row before has left
-    float gt = 1.f;
-    if (token) {
-      float g1[1];
-      load_param<T, 1>(p.gate, p.gate_f32, t * p.gate_stride, g1);
-      gt = g1[0];
-    }
-    const float ry = POST ? p.rstd[t] : 1.f, rh = NEXT ? p.rstd[p.T + t] : 0.f;
-    const f32x2 alpha2 = both(p.alpha), rh2 = both(rh), yg2 = both(ry * gt);
-    f32x2 h[NV][N2], e[NV][N2];
+    const float ry = ahead.ry, rh = ahead.rh, gt = ahead.gt;
+    ahead = scalars(t + step);
+    // h is carried as h rstd(h), the form in which the weights' sum and the correction along h take it
+    const f32x2 rh2 = both(rh), alpha_h = both(p.alpha * rh), yg_h = both(ry * gt * rh);
+    f32x2 h[NEXT ? NV : 1][N2], e[NV][N2];
     f32x2 s0 = both(0.f), s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -514,7 +551,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
         // v = w y (g): what the norm's sum takes the gradient times
         unpack16(lds16(src), v, T());
         if (POST) {
-          load_piece<T, P>(p.w, tid + i * tpr, f);
+          weight_of(i, f);
 #pragma unroll
           for (int j = 0; j < N2; ++j) v[j] = mul2(v[j], f[j]);
         }
@@ -523,29 +560,37 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
 #pragma unroll
           for (int j = 0; j < N2; ++j) v[j] = mul2(v[j], f[j]);
         }
-        if (res) {
-          unpack16(lds16(src + at_r), f, T());
-#pragma unroll
-          for (int j = 0; j < N2; ++j) h[i][j] = fma2(v[j], yg2, mul2(f[j], alpha2));
-        } else {
-#pragma unroll
-          for (int j = 0; j < N2; ++j) h[i][j] = mul2(v[j], yg2);
-        }
         if (has_dh) {
           unpack16(lds16(src + at_h), e[i], T());
         } else {
 #pragma unroll
           for (int j = 0; j < N2; ++j) e[i][j] = both(0.f);
         }
-        if (has_dn) {
-          f32x2 d[N2];
-          unpack16(lds16(src + at_n), d, T());
-          load_piece<T, P>(p.wn, tid + i * tpr, f);
+        if (NEXT) {
+          if (res) {
+            unpack16(lds16(src + at_r), f, T());
 #pragma unroll
-          for (int j = 0; j < N2; ++j) {
-            d[j] = mul2(d[j], f[j]);
-            e[i][j] = fma2(d[j], rh2, e[i][j]);
-            s0 = fma2(d[j], h[i][j], s0);
+            for (int j = 0; j < N2; ++j) h[i][j] = fma2(v[j], yg_h, mul2(f[j], alpha_h));
+          } else {
+#pragma unroll
+            for (int j = 0; j < N2; ++j) h[i][j] = mul2(v[j], yg_h);
+          }
+          if (has_dn) {
+            f32x2 d[N2];
+            unpack16(lds16(src + at_n), d, T());
+            if (HOLD) {
+#pragma unroll
+              for (int j = 0; j < N2; ++j) f[j] = hold_n[HOLD ? i : 0][j];
+            } else {
+              load_piece<T, P>(p.wn, tid + i * tpr, f);
+            }
+#pragma unroll
+            for (int j = 0; j < N2; ++j) {
+              an[i][j] = fma2(d[j], h[i][j], an[i][j]);
+              d[j] = mul2(d[j], f[j]);
+              e[i][j] = fma2(d[j], rh2, e[i][j]);
+              s0 = fma2(d[j], h[i][j], s0);
+            }
           }
         }
 #pragma unroll
@@ -556,14 +601,14 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
       }
     float t0 = both_of(s0), t1 = both_of(s1), t2 = both_of(s2);
     if (POST || NEXT || token) red.sum3(t0, t1, t2);
-    const float c3 = NEXT ? rh * rh * rh * t0 * inv_h : 0.f;
-    const float raw = t1 - c3 * t2;
+    const float c1 = NEXT ? rh * t0 * inv_h : 0.f;          // rstd(h)^3 mean(w' dn h) h = c1 (h rstd(h))
+    const float raw = t1 - c1 * t2;
     const float cy = POST ? ry * ry * ry * gt * raw * inv_h : 0.f;
     if (token && tid == 0 && b.dgate != nullptr) {
       const float one[1] = {ry * raw};
       store_param<T, 1>(b.dgate, p.gate_f32, t, one);
     }
-    const f32x2 c32 = both(-c3), cy2 = both(-cy), ry2 = both(ry);
+    const f32x2 c2 = both(-c1), cy2 = both(-cy), alpha2 = both(p.alpha), yg2 = both(ry * gt);
     uint4* dyo = reinterpret_cast<uint4*>(static_cast<T*>(b.dy) + t * p.H) + tid;
     uint4* dro = reinterpret_cast<uint4*>(static_cast<T*>(b.dr) + t * p.H) + tid;
     uint4* dgo = reinterpret_cast<uint4*>(static_cast<T*>(b.dgate) + t * p.H) + tid;
@@ -572,42 +617,36 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
       if (tid + i * tpr < chunks) {
         const uint32_t src = at + (uint32_t)(i * tpr) * 16;
         f32x2 y[N2], f[N2], d[N2];
-        if (has_dn) {
-          unpack16(lds16(src + at_n), f, T());
 #pragma unroll
-          for (int j = 0; j < N2; ++j) an[i][j] = fma2(f[j], mul2(h[i][j], rh2), an[i][j]);
-        }
-#pragma unroll
-        for (int j = 0; j < N2; ++j) d[j] = NEXT ? fma2(h[i][j], c32, e[i][j]) : e[i][j];
+        for (int j = 0; j < N2; ++j) d[j] = NEXT ? fma2(h[i][j], c2, e[i][j]) : e[i][j];
         if (b.dr != nullptr) {
 #pragma unroll
           for (int j = 0; j < N2; ++j) f[j] = mul2(d[j], alpha2);
           dro[i * tpr] = pack16(f, T());
         }
         unpack16(lds16(src), y, T());
-        if (GATE == 0) {
-#pragma unroll
-          for (int j = 0; j < N2; ++j) d[j] = mul2(d[j], both(gt));
-        }
-        if (POST) load_piece<T, P>(p.w, tid + i * tpr, f);
+        if (POST) weight_of(i, f);
         if (GATE != 0) {
           f32x2 g[N2], dg[N2];
           if (GATE == 1) load_gate_piece<T>(p, tid + i * tpr, g); else unpack16(lds16(src + at_g), g, T());
 #pragma unroll
           for (int j = 0; j < N2; ++j) {
-            const f32x2 u = POST ? mul2(mul2(y[j], ry2), f[j]) : y[j];
+            const f32x2 u = POST ? mul2(mul2(y[j], yg2), f[j]) : y[j];          // (gt is 1 here)
             if (GATE == 1) ag[i][j] = fma2(d[j], u, ag[i][j]); else dg[j] = mul2(d[j], u);
             d[j] = mul2(d[j], g[j]);
           }
           if (GATE == 2 && b.dgate != nullptr) dgo[i * tpr] = pack16(dg, T());
         }
-        // d is the gradient of u now
+        // d times a token's gate is the gradient of u
         if (POST) {
 #pragma unroll
           for (int j = 0; j < N2; ++j) {
-            aw[i][j] = fma2(d[j], mul2(y[j], ry2), aw[i][j]);
-            d[j] = fma2(d[j], mul2(f[j], ry2), mul2(y[j], cy2));
+            aw[i][j] = fma2(d[j], mul2(y[j], yg2), aw[i][j]);
+            d[j] = fma2(d[j], mul2(f[j], yg2), mul2(y[j], cy2));
           }
+        } else if (GATE == 0) {
+#pragma unroll
+          for (int j = 0; j < N2; ++j) d[j] = mul2(d[j], yg2);
         }
         if (b.dy != nullptr) dyo[i * tpr] = pack16(d, T());
       }
@@ -707,16 +746,17 @@ void (*fwd_ring(const NormParams& p, bool hold))(NormParams) {
   if (p.w != nullptr) return hold ? fwd_ring_g<T, P, true, true>(g) : fwd_ring_g<T, P, true, false>(g);
   return hold ? fwd_ring_g<T, P, false, true>(g) : fwd_ring_g<T, P, false, false>(g);
 }
-template <typename T, typename P, int GATE>
+template <typename T, typename P, int GATE, bool HOLD>
 void (*bwd_ring_g(const NormParams& p))(NormBwdParams) {
   if (p.w != nullptr)
-    return p.wn != nullptr ? block_norm_bwd_ring_kernel<T, P, GATE, true, true> : block_norm_bwd_ring_kernel<T, P, GATE, true, false>;
-  return p.wn != nullptr ? block_norm_bwd_ring_kernel<T, P, GATE, false, true> : block_norm_bwd_ring_kernel<T, P, GATE, false, false>;
+    return p.wn != nullptr ? block_norm_bwd_ring_kernel<T, P, GATE, true, true, HOLD> : block_norm_bwd_ring_kernel<T, P, GATE, true, false, HOLD>;
+  return p.wn != nullptr ? block_norm_bwd_ring_kernel<T, P, GATE, false, true, HOLD> : block_norm_bwd_ring_kernel<T, P, GATE, false, false, false>;
 }
 template <typename T, typename P>
 void (*bwd_ring(const NormParams& p))(NormBwdParams) {
   const int g = ring_gate(p);
-  return g == 0 ? bwd_ring_g<T, P, 0>(p) : g == 1 ? bwd_ring_g<T, P, 1>(p) : bwd_ring_g<T, P, 2>(p);
+  if (g == 0) return bwd_ring_g<T, P, 0, true>(p);
+  return g == 1 ? bwd_ring_g<T, P, 1, false>(p) : bwd_ring_g<T, P, 2, false>(p);
 }
 
 template <typename T>
@@ -775,7 +815,7 @@ int launch_norm_bwd_t(const NormBwdParams& b, const ColumnSumParams& sums, cudaS
                    (p.gate_kind == B200MOE_GATE_TOKEN || aligned16(b.dgate));
   BwdShape r = bwd_shape<T>(p, vec);
   constexpr int NV = 16 / V;
-  const int arrays = 1 + (p.r != nullptr) + (b.dh != nullptr) + (b.dn != nullptr) + (p.gate_kind == B200MOE_GATE_FULL);
+  const int arrays = 1 + (p.wn != nullptr && p.r != nullptr) + (b.dh != nullptr) + (b.dn != nullptr) + (p.gate_kind == B200MOE_GATE_FULL);
   const int row_bytes = arrays * p.H * (int)sizeof(T);
   const int tpr = (int)round_up64((p.H / V + NV - 1) / NV, 32);
   const bool ring = ring_ok<T>(p, vec) && tpr <= kRowThreads && 2 * row_bytes <= kRingLimit;
