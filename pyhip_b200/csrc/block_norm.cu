@@ -154,7 +154,7 @@ __device__ __forceinline__ void load_gate_piece(const NormParams& p, int c, f32x
   if (p.gate_f32) load_piece<T, float>(p.gate, c, o); else load_piece<T, T>(p.gate, c, o);
 }
 
-// Forward over a ring of two rows in shared memory, 16-byte pieces and pairs of values throughout, 16 values to a thread.
+// Forward over a ring of two to four rows in shared memory, 16-byte pieces and pairs of values throughout, 16 values to a thread.
 // GATE: 0 none or per token, 1 per channel, 2 per element.  P: type of the norms' weights.
 // HOLD: the weights (times the gate per channel) stay in registers over the rows.  L1 would serve them at every row, which
 // costs it as much as the rows themselves (66 % of its data pipe with fp32 weights; 43.8 -> 36.8 us at 8192 x 2880).  It takes
@@ -164,7 +164,7 @@ constexpr int kNormValues = 16;
 constexpr int kHoldThreads = 768, kNoHoldThreads = 1024;      // of an SM
 template <typename T, typename P, bool POST, int GATE, bool HOLD>
 __global__ void __launch_bounds__(HOLD ? kHoldThreads : kNoHoldThreads, 1)
-block_norm_ring_kernel(const __grid_constant__ NormParams p) {
+block_norm_ring_kernel(const __grid_constant__ NormParams p, int stages) {
   constexpr int VEC = 16 / sizeof(T), NV = kNormValues / VEC, N2 = VEC / 2;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ __align__(16) float slots[2 * 32 * 4];
@@ -207,7 +207,9 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
     }
   };
   const int64_t step = gridDim.x;
-  fetch(blockIdx.x, mine);
+  const uint32_t end = mine + stages * stage_bytes;
+  uint32_t at = mine, other = mine;               // the present row, and the stage that the row before has left
+  for (int s = 0; s < stages - 1; ++s, other += stage_bytes) fetch(blockIdx.x + s * step, other);
   f32x2 hold_f[HOLD ? NV : 1][N2], hold_n[HOLD ? NV : 1][N2];
   if (HOLD) {
 #pragma unroll
@@ -224,10 +226,9 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
     return g[0];
   };
   float next_gate = token_gate(blockIdx.x);       // a row ahead, as the rows themselves
-  uint32_t at = mine, other = mine + stage_bytes;
   for (int64_t t = blockIdx.x; t < p.T; t += step) {
-    copy_wait<0>();
-    fetch(t + step, other);                       // the stage that the row before has left
+    if (stages == 2) copy_wait<0>(); else if (stages == 3) copy_wait<1>(); else copy_wait<2>();
+    fetch(t + (stages - 1) * step, other);
     f32x2 h[NV][N2];
     float scale = 1.f;                            // rstd(y) and a token's gate
     const float gt = next_gate;
@@ -321,9 +322,8 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p) {
           }
         }
     }
-    const uint32_t swap = at;
-    at = other;
-    other = swap;
+    at = at + stage_bytes == end ? mine : at + stage_bytes;
+    other = other + stage_bytes == end ? mine : other + stage_bytes;
   }
 }
 
@@ -446,12 +446,16 @@ block_norm_bwd_kernel(const __grid_constant__ NormBwdParams b) {
 }
 
 // Backward over a ring of rows in shared memory.  What a row needs twice (y, dn) is read from there again instead of held,
-// so that 16 values a thread and their sums over tokens fit the registers.  GATE and P as in the forward kernel.
-// HOLD: the weights stay in registers over the rows (a gate's values leave no room for them).
-template <typename T, typename P, int GATE, bool POST, bool NEXT, bool HOLD>
-__global__ void __launch_bounds__(kRowThreads, 1)
+// so that a thread's values and their sums over tokens fit the registers.  GATE and P as in the forward kernel.
+// VALUES of a row to a thread: 16, and where two CTAs of those would not fit an SM (rows of more than 4096 values), 8 in up
+// to 896 threads, since the one CTA's phases between its barriers need the warps (4096 x 7168: 79 against 88 us; a gate's
+// values and their sums do not fit there).  Weights held in registers cost more in occupancy than their loads do
+// (8192 x 4096: 90 against 80 us).
+constexpr int kWideThreads = 896;
+template <typename T, typename P, int GATE, bool POST, bool NEXT, int VALUES>
+__global__ void __launch_bounds__(VALUES == 8 ? kWideThreads : kRowThreads, 1)
 block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
-  constexpr int VEC = 16 / sizeof(T), NV = 16 / VEC, N2 = VEC / 2;
+  constexpr int VEC = 16 / sizeof(T), NV = VALUES / VEC, N2 = VEC / 2;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ __align__(16) float slots[2 * 32 * 4];
   const NormParams& p = b.f;
@@ -515,23 +519,6 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
     }
     return r;
   };
-  f32x2 hold_w[HOLD && POST ? NV : 1][N2], hold_n[HOLD && NEXT ? NV : 1][N2];
-  if (HOLD) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (tid + i * tpr < chunks) {
-        if (POST) load_piece<T, P>(p.w, tid + i * tpr, hold_w[i]);
-        if (NEXT) load_piece<T, P>(p.wn, tid + i * tpr, hold_n[i]);
-      }
-  }
-  auto weight_of = [&](int i, f32x2 (&f)[N2]) {
-    if (HOLD) {
-#pragma unroll
-      for (int j = 0; j < N2; ++j) f[j] = hold_w[HOLD && POST ? i : 0][j];
-    } else {
-      load_piece<T, P>(p.w, tid + i * tpr, f);
-    }
-  };
   RowScalars ahead = scalars(blockIdx.x);
   uint32_t at = mine, other = mine + stage_bytes;
   for (int64_t t = blockIdx.x; t < p.T; t += step) {
@@ -551,7 +538,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
         // v = w y (g): what the norm's sum takes the gradient times
         unpack16(lds16(src), v, T());
         if (POST) {
-          weight_of(i, f);
+          load_piece<T, P>(p.w, tid + i * tpr, f);
 #pragma unroll
           for (int j = 0; j < N2; ++j) v[j] = mul2(v[j], f[j]);
         }
@@ -578,12 +565,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
           if (has_dn) {
             f32x2 d[N2];
             unpack16(lds16(src + at_n), d, T());
-            if (HOLD) {
-#pragma unroll
-              for (int j = 0; j < N2; ++j) f[j] = hold_n[HOLD ? i : 0][j];
-            } else {
-              load_piece<T, P>(p.wn, tid + i * tpr, f);
-            }
+            load_piece<T, P>(p.wn, tid + i * tpr, f);
 #pragma unroll
             for (int j = 0; j < N2; ++j) {
               an[i][j] = fma2(d[j], h[i][j], an[i][j]);
@@ -625,7 +607,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
           dro[i * tpr] = pack16(f, T());
         }
         unpack16(lds16(src), y, T());
-        if (POST) weight_of(i, f);
+        if (POST) load_piece<T, P>(p.w, tid + i * tpr, f);
         if (GATE != 0) {
           f32x2 g[N2], dg[N2];
           if (GATE == 1) load_gate_piece<T>(p, tid + i * tpr, g); else unpack16(lds16(src + at_g), g, T());
@@ -688,6 +670,7 @@ column_sum_kernel(const __grid_constant__ ColumnSumParams p) {
   if (p.dst[which] == nullptr) return;
   float a = 0.f;
   if (col < p.H)
+#pragma unroll 8
     for (int r = grp; r < p.rows; r += 8) a += p.part[((int64_t)r * 3 + which) * p.H + col];
   s[grp][threadIdx.x & 31] = a;
   __syncthreads();
@@ -736,27 +719,27 @@ int ring_gate(const NormParams& p) {
   return p.gate_kind == B200MOE_GATE_CHANNEL ? 1 : p.gate_kind == B200MOE_GATE_FULL ? 2 : 0;
 }
 template <typename T, typename P, bool POST, bool HOLD>
-void (*fwd_ring_g(int g))(NormParams) {
+void (*fwd_ring_g(int g))(NormParams, int) {
   return g == 0 ? block_norm_ring_kernel<T, P, POST, 0, HOLD> : g == 1 ? block_norm_ring_kernel<T, P, POST, 1, HOLD>
                                                                       : block_norm_ring_kernel<T, P, POST, 2, HOLD>;
 }
 template <typename T, typename P>
-void (*fwd_ring(const NormParams& p, bool hold))(NormParams) {
+void (*fwd_ring(const NormParams& p, bool hold))(NormParams, int) {
   const int g = ring_gate(p);
   if (p.w != nullptr) return hold ? fwd_ring_g<T, P, true, true>(g) : fwd_ring_g<T, P, true, false>(g);
   return hold ? fwd_ring_g<T, P, false, true>(g) : fwd_ring_g<T, P, false, false>(g);
 }
-template <typename T, typename P, int GATE, bool HOLD>
+template <typename T, typename P, int GATE, int VALUES>
 void (*bwd_ring_g(const NormParams& p))(NormBwdParams) {
   if (p.w != nullptr)
-    return p.wn != nullptr ? block_norm_bwd_ring_kernel<T, P, GATE, true, true, HOLD> : block_norm_bwd_ring_kernel<T, P, GATE, true, false, HOLD>;
-  return p.wn != nullptr ? block_norm_bwd_ring_kernel<T, P, GATE, false, true, HOLD> : block_norm_bwd_ring_kernel<T, P, GATE, false, false, false>;
+    return p.wn != nullptr ? block_norm_bwd_ring_kernel<T, P, GATE, true, true, VALUES> : block_norm_bwd_ring_kernel<T, P, GATE, true, false, VALUES>;
+  return p.wn != nullptr ? block_norm_bwd_ring_kernel<T, P, GATE, false, true, VALUES> : block_norm_bwd_ring_kernel<T, P, GATE, false, false, VALUES>;
 }
 template <typename T, typename P>
-void (*bwd_ring(const NormParams& p))(NormBwdParams) {
+void (*bwd_ring(const NormParams& p, bool wide))(NormBwdParams) {
   const int g = ring_gate(p);
-  if (g == 0) return bwd_ring_g<T, P, 0, true>(p);
-  return g == 1 ? bwd_ring_g<T, P, 1, false>(p) : bwd_ring_g<T, P, 2, false>(p);
+  if (g == 0) return wide ? bwd_ring_g<T, P, 0, 8>(p) : bwd_ring_g<T, P, 0, 16>(p);
+  return g == 1 ? bwd_ring_g<T, P, 1, 16>(p) : bwd_ring_g<T, P, 2, 16>(p);
 }
 
 template <typename T>
@@ -767,14 +750,19 @@ int launch_norm_t(const NormParams& p, cudaStream_t st) {
     constexpr int NV = kNormValues / V;
     const int tpr = (int)round_up64((p.H / V + NV - 1) / NV, 32);
     const int arrays = 1 + (p.r != nullptr) + (p.gate_kind == B200MOE_GATE_FULL);
-    const int smem = 2 * arrays * p.H * (int)sizeof(T);
-    if (smem <= kRingLimit && tpr <= kNoHoldThreads) {
+    const int row_bytes = arrays * p.H * (int)sizeof(T);
+    if (2 * row_bytes <= kRingLimit && tpr <= kNoHoldThreads) {
       const bool hold = 2 * tpr <= kHoldThreads;
-      const int per_sm = std::max(1, std::min((hold ? kHoldThreads : kNoHoldThreads) / tpr, kRingLimit / (smem + 2048)));
+      const int per_sm = std::max(1, std::min((hold ? kHoldThreads : kNoHoldThreads) / tpr, kRingLimit / (2 * row_bytes + 2048)));
+      // Rows ahead until an SM has 40 KB on their way, which its share of the memory's rate times the latency asks for
+      // (the quantiser at 16384 x 4096, 24 KB with one row ahead).
+      const int ahead = std::min((40 * 1024 + per_sm * row_bytes - 1) / (per_sm * row_bytes), 3);
+      const int stages = std::max(2, std::min(ahead + 1, kRingLimit / per_sm / row_bytes));
+      const size_t smem = (size_t)stages * row_bytes;
       const int grid = (int)std::min<int64_t>(p.T, (int64_t)device_sm_count() * per_sm);
-      void (*k)(NormParams) = fp32_weights(p) ? fwd_ring<T, float>(p, hold) : fwd_ring<T, T>(p, hold);
+      void (*k)(NormParams, int) = fp32_weights(p) ? fwd_ring<T, float>(p, hold) : fwd_ring<T, T>(p, hold);
       B200_CHECK_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingLimit));
-      B200_CHECK_CUDA(launch_chained(k, dim3(grid), dim3(tpr), smem, st, p));
+      B200_CHECK_CUDA(launch_chained(k, dim3(grid), dim3(tpr), smem, st, p, stages));
       return 0;
     }
   }
@@ -814,17 +802,18 @@ int launch_norm_bwd_t(const NormBwdParams& b, const ColumnSumParams& sums, cudaS
   const bool vec = vector_ok<T>(p) && aligned16(b.dh) && aligned16(b.dn) && aligned16(b.dy) && aligned16(b.dr) &&
                    (p.gate_kind == B200MOE_GATE_TOKEN || aligned16(b.dgate));
   BwdShape r = bwd_shape<T>(p, vec);
-  constexpr int NV = 16 / V;
+  const bool wide = 2 * ((p.H + 15) / 16) > kRowThreads && (p.H + 7) / 8 <= kWideThreads && ring_gate(p) == 0;
+  const int values = wide ? 8 : 16, threads = wide ? kWideThreads : kRowThreads;
   const int arrays = 1 + (p.wn != nullptr && p.r != nullptr) + (b.dh != nullptr) + (b.dn != nullptr) + (p.gate_kind == B200MOE_GATE_FULL);
   const int row_bytes = arrays * p.H * (int)sizeof(T);
-  const int tpr = (int)round_up64((p.H / V + NV - 1) / NV, 32);
-  const bool ring = ring_ok<T>(p, vec) && tpr <= kRowThreads && 2 * row_bytes <= kRingLimit;
+  const int tpr = (int)round_up64((p.H + values - 1) / values, 32);
+  const bool ring = ring_ok<T>(p, vec) && tpr <= threads && 2 * row_bytes <= kRingLimit;
   void (*k)(NormBwdParams) = nullptr;
   if (ring) {
-    const int per_sm = std::max(1, std::min(kRowThreads / tpr, kRingLimit / (2 * row_bytes + 2048)));
+    const int per_sm = std::max(1, std::min(threads / tpr, kRingLimit / (2 * row_bytes + 2048)));
     r.grid = (int)std::min<int64_t>(p.T, (int64_t)device_sm_count() * per_sm);
     r.s.rows = 1;
-    void (*kr)(NormBwdParams) = fp32_weights(p) ? bwd_ring<T, float>(p) : bwd_ring<T, T>(p);
+    void (*kr)(NormBwdParams) = fp32_weights(p) ? bwd_ring<T, float>(p, wide) : bwd_ring<T, T>(p, wide);
     B200_CHECK_CUDA(cudaFuncSetAttribute(kr, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingLimit));
     B200_CHECK_CUDA(launch_chained(kr, dim3(r.grid), dim3(tpr), 2 * (size_t)row_bytes, st, b));
   } else if (vec)
