@@ -154,6 +154,28 @@ __device__ __forceinline__ void load_gate_piece(const NormParams& p, int c, f32x
   if (p.gate_f32) load_piece<T, float>(p.gate, c, o); else load_piece<T, T>(p.gate, c, o);
 }
 
+// a thread's pieces of row t as 8-bit integers, and the row's scale, from the bits of its largest magnitude
+template <typename T, int NV, int N2>
+__device__ __forceinline__ void store_int8_row(const NormParams& p, int64_t t, uint32_t amax_bits, const f32x2 (&v)[NV][N2], int chunks) {
+  constexpr int VEC = 2 * N2;
+  const int tid = (int)threadIdx.x, tpr = (int)blockDim.x;
+  const float s = int8_scale(amax_bits), inv = __fdividef(1.f, s);       // (quant_int8 needs no exact reciprocal)
+  const bool bad = amax_bits >= 0x7f800000u;
+  if (tid == 0) p.q_scale[t] = s;
+  uint8_t* out = reinterpret_cast<uint8_t*>(p.q + t * p.H) + tid * VEC;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (tid + i * tpr < chunks) {
+      uint32_t k[N2 / 2];
+      quant_int8(v[i], s, inv, k);
+      if constexpr (N2 == 4) {
+        *reinterpret_cast<uint2*>(out + i * tpr * VEC) = bad ? make_uint2(0, 0) : make_uint2(k[0], k[1]);
+      } else {
+        *reinterpret_cast<uint32_t*>(out + i * tpr * VEC) = bad ? 0u : k[0];
+      }
+    }
+}
+
 // Forward over a ring of two to four rows in shared memory, 16-byte pieces and pairs of values throughout, 16 values to a thread.
 // GATE: 0 none or per token, 1 per channel, 2 per element.  P: type of the norms' weights.
 // HOLD: the weights (times the gate per channel) stay in registers over the rows.  L1 would serve them at every row, which
@@ -305,23 +327,53 @@ block_norm_ring_kernel(const __grid_constant__ NormParams p, int stages) {
       for (int i = 0; i < NV; ++i)
         if (tid + i * tpr < chunks) amax = max_abs_nan(amax, h[i]);
       const uint32_t m = red.max_u32(__float_as_uint(amax) & 0x7fffffffu);
-      const float sc = int8_scale(m);
-      const bool bad = m >= 0x7f800000u;
-      const float inv = __frcp_rn(sc);
-      if (tid == 0) p.q_scale[t] = sc;
-      uint8_t* qo = reinterpret_cast<uint8_t*>(p.q + t * p.H) + tid * VEC;
+      store_int8_row<T>(p, t, m, h, chunks);
+    }
+    at = at + stage_bytes == end ? mine : at + stage_bytes;
+    other = other + stage_bytes == end ? mine : other + stage_bytes;
+  }
+}
+
+// The token quantiser by itself over the same ring: no norm in between, so 32 values to a thread, which halves what a row
+// costs whatever its width (reduction, scale, copies).
+constexpr int kQuantValues = 32, kQuantThreads = 768;      // of an SM
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads, 1)
+quant_ring_kernel(const __grid_constant__ NormParams p, int stages) {
+  constexpr int VEC = 16 / sizeof(T), NV = kQuantValues / VEC, N2 = VEC / 2;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ __align__(16) float slots[2 * 32 * 4];
+  CtaReduce red(slots);
+  grid_dep_wait();
+  grid_dep_launch();
+  const int chunks = p.H / VEC, tpr = (int)blockDim.x, tid = (int)threadIdx.x;
+  const uint32_t stage_bytes = (uint32_t)chunks * 16;
+  const uint32_t mine = smem_u32(ring) + (uint32_t)tid * 16, end = mine + stages * stage_bytes;
+  auto fetch = [&](int64_t t, uint32_t at) {
+    if (t < p.T) {
+      const uint4* y = reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + t * p.y_stride) + tid;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (tid + i * tpr < chunks) {
-          uint32_t k[N2 / 2];
-          quant_int8(h[i], sc, inv, k);
-          if constexpr (N2 == 4) {
-            *reinterpret_cast<uint2*>(qo + i * tpr * VEC) = bad ? make_uint2(0, 0) : make_uint2(k[0], k[1]);
-          } else {
-            *reinterpret_cast<uint32_t*>(qo + i * tpr * VEC) = bad ? 0u : k[0];
-          }
-        }
+        if (tid + i * tpr < chunks) copy16_async(at + (uint32_t)(i * tpr) * 16, y + i * tpr);
     }
+    copy_commit();
+  };
+  const int64_t step = gridDim.x;
+  uint32_t at = mine, other = mine;
+  for (int s = 0; s < stages - 1; ++s, other += stage_bytes) fetch(blockIdx.x + s * step, other);
+  for (int64_t t = blockIdx.x; t < p.T; t += step) {
+    if (stages == 2) copy_wait<0>(); else if (stages == 3) copy_wait<1>(); else copy_wait<2>();
+    fetch(t + (stages - 1) * step, other);
+    f32x2 v[NV][N2];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + i * tpr < chunks) {
+        unpack16(lds16(at + (uint32_t)(i * tpr) * 16), v[i], T());
+        amax = max_abs_nan(amax, v[i]);
+      }
+    const uint32_t m = red.max_u32(__float_as_uint(amax) & 0x7fffffffu);
+    store_int8_row<T>(p, t, m, v, chunks);
     at = at + stage_bytes == end ? mine : at + stage_bytes;
     other = other + stage_bytes == end ? mine : other + stage_bytes;
   }
@@ -746,6 +798,17 @@ template <typename T>
 int launch_norm_t(const NormParams& p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = vector_ok<T>(p);
+  if (ring_ok<T>(p, vec) && p.r == nullptr && p.w == nullptr && p.wn == nullptr && p.gate_kind == B200MOE_GATE_NONE && p.h == nullptr) {
+    constexpr int NV = kQuantValues / V;
+    const int tpr = (int)round_up64((p.H / V + NV - 1) / NV, 32), row_bytes = p.H * (int)sizeof(T);
+    const int per_sm = std::max(1, std::min(kQuantThreads / tpr, kRingLimit / (2 * row_bytes + 2048)));
+    const int ahead = std::min((40 * 1024 + per_sm * row_bytes - 1) / (per_sm * row_bytes), 3);
+    const int stages = std::max(2, std::min(ahead + 1, kRingLimit / per_sm / row_bytes));
+    const int grid = (int)std::min<int64_t>(p.T, (int64_t)device_sm_count() * per_sm);
+    B200_CHECK_CUDA(cudaFuncSetAttribute(quant_ring_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingLimit));
+    B200_CHECK_CUDA(launch_chained(quant_ring_kernel<T>, dim3(grid), dim3(tpr), (size_t)stages * row_bytes, st, p, stages));
+    return 0;
+  }
   if (ring_ok<T>(p, vec)) {
     constexpr int NV = kNormValues / V;
     const int tpr = (int)round_up64((p.H / V + NV - 1) / NV, 32);

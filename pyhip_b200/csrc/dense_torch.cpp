@@ -228,6 +228,8 @@ NormOutputs norm_forward(const Tensor& y, const OptTensor& residual, const OptTe
 // Gradients of a backward pass that is itself being recorded: nothing here can be differentiated again, and says so.
 variable_list once(variable_list grads, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads)
+    if (g.defined()) g.set_requires_grad(true);     // so that the node below stands behind them
   auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is not twice differentiable", (int64_t)grads.size());
   return (*node)(std::move(grads));
 }

@@ -45,6 +45,20 @@ def test_quantiser_is_exact(T, K, dtype):
     _equal((torch.randn(T, K, generator=g) * 3).to(dtype).to(DEV))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,K", [(593, 512), (700, 1040), (2000, 2880), (600, 16384), (600, 15)])
+def test_quantiser_is_exact_for_many_rows(T, K, dtype):
+    g = torch.Generator().manual_seed(T + K)
+    x = torch.randn(T, K, generator=g) * torch.logspace(-30, 30, T)[:, None].clamp(1e-4 if dtype == torch.float16 else 0, 1e3 if dtype == torch.float16 else 1e31)
+    x[3], x[4, 5], x[5, 6], x[-1, -1] = 0, float("inf"), float("nan"), float("-inf")
+    half = (torch.arange(K) % 254 - 126.5).roll(1)
+    x[7], x[8] = half, half * 3 * 2 ** -4                  # ties, exactly, where the row's largest value is 127 scales
+    x[7, 0], x[8, 0] = 127, 127 * 3 * 2 ** -4
+    x = x.to(dtype).to(DEV)
+    _equal(x)
+    _equal(torch.cat([x, x], dim=1)[:, 8:K + 8] if K % 8 == 0 else x)
+
+
 def test_quantiser_at_the_borders():
     """Rows whose quotients are ties (scale a power of two, or 3 times one, which is exact in fp16), next to ties, zeros, tiny,
     subnormal and huge values, infinities and NaN."""
