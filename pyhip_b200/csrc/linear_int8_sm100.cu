@@ -5,9 +5,10 @@
 // Two kernels, chosen by size (pick_variant):
 //   split   one 128-feature x BT-token tile per CTA, the weights on the MMA's M side; the CTAs of a cluster take equal
 //           ranges of K and add their tiles through distributed shared memory.  For few tokens, where the weights' bytes
-//           and the launch latency bound the call: every weight byte is requested as soon as the CTA starts.  A handful of
-//           tokens are quantised here too, by the epilogue warps while the weights are on their way: every CTA reads the
-//           rows for their scales and converts its own range of K (one launch instead of two, and no workspace).
+//           and the launch latency bound the call: every weight byte is requested as soon as the CTA starts.  A single
+//           token is quantised here too, by the epilogue warps while the weights are on their way: every CTA reads the row
+//           for its scale and converts its own range of K (one launch instead of two and no workspace, the same time on
+//           the GPU, 3.3 us less on the host; from two tokens on the repeated reading costs the GPU more).
 //   pair    persistent CTA pairs (cta_group::2), 256 tokens x BN features a tile: each CTA holds its 128 tokens' rows and
 //           half of the feature rows, two accumulators overlap a tile's epilogue with the next one's products.
 //
@@ -46,8 +47,7 @@ struct LinearParams {
   const float* bias;
   void* y;
   int32_t* status;
-  const void* x;        // rows that the split kernel quantises itself
-  int64_t x_stride;
+  const void* x;        // the row that the split kernel quantises itself
   int T, N, K, KB, k_tail_steps, stages, fp16, store_tma, early_weights, x_dtype, x_vec;
   int tokens, splits;             // split: token tile, CTAs that share K
   int m_tiles, n_tiles;           // pair
@@ -153,8 +153,7 @@ __device__ __forceinline__ void drain_copies(SmemCtlI8* ctl, int64_t issued, int
 }
 
 // ------------------------------------------------------------------------------------ split
-constexpr int kFusedTokens = 8;                 // rows that the split kernel quantises itself, at most
-constexpr int kFusedTile = 16;                  // token tile of the MMA then
+constexpr int kFusedTile = 16;                  // token tile of the MMA where the split kernel quantises its one row itself
 constexpr int kFusedBlockBytes = kFusedTile * kTileKI8;
 constexpr int kFusedBlocks = 16;                // k-blocks of a CTA, at most
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -176,41 +175,36 @@ __device__ __forceinline__ void load_16(const T* src, bool vec, f32x2 (&v)[8]) {
     for (int i = 0; i < 8; ++i) v[i] = pair(to_f(src[2 * i]), to_f(src[2 * i + 1]));
   }
 }
-// The epilogue warps' part of the fused split kernel: scales of all rows, then this CTA's k-blocks of them as the MMA's N-side
-// tiles (16 rows of 128 bytes in the 128-byte swizzle; rows beyond T are zero).
+// The epilogue warps' part of the fused split kernel: the row's scale, then this CTA's k-blocks of the row as the MMA's N-side
+// tiles (16 rows of 128 bytes in the 128-byte swizzle, all but the first of them zero).
 template <typename T>
-__device__ __forceinline__ void quantise_rows(const LinearParams& p, uint32_t tiles, int kb0, int blocks, uint32_t* maxima, float* scales) {
-  const int te = (int)threadIdx.x - 64, warp = te >> 5;
+__device__ __forceinline__ void quantise_row(const LinearParams& p, uint32_t tiles, int kb0, int blocks, uint32_t* maxima, float* scale) {
+  const int te = (int)threadIdx.x - 64;
   const T* x = static_cast<const T*>(p.x);
   const bool vec = p.x_vec != 0;
-  const int pieces = p.K / 16;
-  for (int t = 0; t < p.T; ++t) {
-    float m = 0.f;
-#pragma unroll 2
-    for (int c = te; c < pieces; c += 128) {
-      f32x2 v[8];
-      load_16<T>(x + t * p.x_stride + c * 16, vec, v);
-      m = max_abs_nan(m, v);
-    }
-    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7fffffffu);
-    if ((te & 31) == 0) maxima[t * 4 + warp] = bits;
+  float m = 0.f;
+#pragma unroll 4
+  for (int c = te; c < p.K / 16; c += 128) {
+    f32x2 v[8];
+    load_16<T>(x + c * 16, vec, v);
+    m = max_abs_nan(m, v);
   }
+  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m) & 0x7fffffffu);
+  if ((te & 31) == 0) maxima[te >> 5] = bits;
+  for (int i = te; i < blocks * (kFusedBlockBytes / 16); i += 128)
+    if ((i & 127) >= 8) st_shared_v4(tiles + (uint32_t)i * 16, 0, 0, 0, 0);          // rows 1 to 15 of each tile
   epilogue_sync();
-  if (te < p.T) scales[te] = int8_scale(max(max(maxima[te * 4], maxima[te * 4 + 1]), max(maxima[te * 4 + 2], maxima[te * 4 + 3])));
-  epilogue_sync();
-  const int per_row = blocks * 8;                          // 16-byte pieces of a row in this CTA's range
-  for (int i = te; i < kFusedTile * per_row; i += 128) {
-    const int t = i / per_row, c = i - t * per_row, k = kb0 * kTileKI8 + c * 16;
+  const float s = int8_scale(max(max(maxima[0], maxima[1]), max(maxima[2], maxima[3])));
+  if (te == 0) *scale = s;
+  for (int c = te; c < blocks * 8; c += 128) {             // 16-byte pieces of the row in this CTA's range
+    const int k = kb0 * kTileKI8 + c * 16;
     uint32_t o[4] = {0, 0, 0, 0};
-    if (t < p.T && k < p.K) {
-      const float s = scales[t];
-      if (s == s) {                                        // (a row with an infinity or NaN: zeros, and scale NaN)
-        f32x2 v[8];
-        load_16<T>(x + t * p.x_stride + k, vec, v);
-        quant_int8(v, s, __frcp_rn(s), o);
-      }
+    if (k < p.K && s == s) {                               // (a row with an infinity or NaN: zeros, and scale NaN)
+      f32x2 v[8];
+      load_16<T>(x + k, vec, v);
+      quant_int8(v, s, __fdividef(1.f, s), o);
     }
-    st_shared_v4(tiles + (uint32_t)(c >> 3) * kFusedBlockBytes + (uint32_t)t * kTileKI8 + (uint32_t)(((c & 7) ^ (t & 7)) << 4), o[0], o[1], o[2], o[3]);
+    st_shared_v4(tiles + (uint32_t)(c >> 3) * kFusedBlockBytes + (uint32_t)((c & 7) << 4), o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -218,8 +212,8 @@ template <bool FUSED>
 __global__ void __launch_bounds__(kThreadsI8)
 linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint32_t maxima[FUSED ? kFusedTokens * 4 : 1];
-  __shared__ float scales[FUSED ? kFusedTokens : 1];
+  __shared__ uint32_t maxima[4];
+  __shared__ float row_scale;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   SmemCtlI8* ctl = reinterpret_cast<SmemCtlI8*>(smem);
   const uint32_t stage0 = smem_u32(smem) + kCtlBytes;
@@ -308,9 +302,9 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
   } else {
     grid_dep_wait();
     if (FUSED) {
-      if (p.x_dtype == B200MOE_T_BF16) quantise_rows<__nv_bfloat16>(p, token_tiles, kb0, kb1 - kb0, maxima, scales);
-      else if (p.x_dtype == B200MOE_T_FP16) quantise_rows<__half>(p, token_tiles, kb0, kb1 - kb0, maxima, scales);
-      else quantise_rows<float>(p, token_tiles, kb0, kb1 - kb0, maxima, scales);
+      if (p.x_dtype == B200MOE_T_BF16) quantise_row<__nv_bfloat16>(p, token_tiles, kb0, kb1 - kb0, maxima, &row_scale);
+      else if (p.x_dtype == B200MOE_T_FP16) quantise_row<__half>(p, token_tiles, kb0, kb1 - kb0, maxima, &row_scale);
+      else quantise_row<float>(p, token_tiles, kb0, kb1 - kb0, maxima, &row_scale);
       fence_proxy_async_smem();
       epilogue_sync();
       if (threadIdx.x == 64) mbar_arrive(smem_u32(&ctl->tmem_empty[0]));
@@ -318,8 +312,20 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
   }
   grid_dep_launch();
 
-  // the tile as [token][feature] int32 in the stages' memory, which the products no longer need
+  // what the sums are multiplied by, on its way while the products are finished: a lane's four features, and the token
+  // columns' scales spread over the lanes (the producer's other lanes have not waited for the launch in front yet)
+  grid_dep_wait();
   const int live = min(BT, p.T - t0);
+  const int n = n0 + lane * 4;
+  float ws[4], bs[4], xs_of[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    ws[j] = n + j < p.N ? p.w_scale[n + j] : 0.f;
+    bs[j] = (p.bias != nullptr && n + j < p.N) ? p.bias[n + j] : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) xs_of[j] = (!FUSED && j * 32 + lane < live) ? p.x_scale[t0 + j * 32 + lane] : 0.f;
+  // the tile as [token][feature] int32 in the stages' memory, which the products no longer need
   if (warp >= 2) {
     ok = mbar_wait(smem_u32(&ctl->tmem_full[0]), 0, abort_word, 0x1300);
     if (ok) {
@@ -339,34 +345,38 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
   tc_fence_before_sync();
   cluster_sync_all();
   tc_fence_after_sync();
-  // token columns are dealt out over the cluster's warps; a lane adds four neighbouring features of all its CTAs
-  const int n = n0 + lane * 4;
-  float ws[4], bs[4];
+  // token columns are dealt out over the cluster's warps; a lane adds four neighbouring features of all its CTAs.  Four
+  // columns at a time: a load from another CTA takes hundreds of cycles.
+  const int stride = C * (kThreadsI8 / 32);
+  for (int c0 = rank + C * warp; c0 < live; c0 += 4 * stride) {
+    int4 a[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    ws[j] = n + j < p.N ? p.w_scale[n + j] : 0.f;
-    bs[j] = (p.bias != nullptr && n + j < p.N) ? p.bias[n + j] : 0.f;
-  }
-  for (int c = rank + C * warp; c < live; c += C * (kThreadsI8 / 32)) {
-    int4 a = make_int4(0, 0, 0, 0);
-    const uint32_t at = stage0 + (uint32_t)c * (kRowTile * 4) + lane * 16;
-#pragma unroll 8
+    for (int q = 0; q < 4; ++q) a[q] = make_int4(0, 0, 0, 0);
     for (int r = 0; r < C; ++r) {
-      const int4 v = ld_peer_v4(peer_smem(at, (uint32_t)r));
-      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+      const uint32_t at = peer_smem(stage0 + (uint32_t)c0 * (kRowTile * 4) + lane * 16, (uint32_t)r);
+      int4 v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = c0 + q * stride < live ? ld_peer_v4(at + (uint32_t)(q * stride) * (kRowTile * 4)) : make_int4(0, 0, 0, 0);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) { a[q].x += v[q].x; a[q].y += v[q].y; a[q].z += v[q].z; a[q].w += v[q].w; }
     }
-    const float xs = FUSED ? scales[c] : p.x_scale[t0 + c];
-    const float o0 = fmaf((float)a.x * xs, ws[0], bs[0]), o1 = fmaf((float)a.y * xs, ws[1], bs[1]);
-    const float o2 = fmaf((float)a.z * xs, ws[2], bs[2]), o3 = fmaf((float)a.w * xs, ws[3], bs[3]);
-    const uint32_t lo = pack2(o0, o1, p.fp16), hi = pack2(o2, o3, p.fp16);
-    uint16_t* dst = static_cast<uint16_t*>(p.y) + (int64_t)(t0 + c) * p.N + n;
-    if ((p.N & 3) == 0) {
-      if (n < p.N) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-    } else {
-      if (n < p.N) dst[0] = (uint16_t)lo;
-      if (n + 1 < p.N) dst[1] = (uint16_t)(lo >> 16);
-      if (n + 2 < p.N) dst[2] = (uint16_t)hi;
-      if (n + 3 < p.N) dst[3] = (uint16_t)(hi >> 16);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = c0 + q * stride;
+      if (c >= live) break;                                  // (the same for the whole warp)
+      const float xs = FUSED ? row_scale : __shfl_sync(0xffffffffu, c < 32 ? xs_of[0] : c < 64 ? xs_of[1] : c < 96 ? xs_of[2] : xs_of[3], c & 31);
+      const float o0 = fmaf((float)a[q].x * xs, ws[0], bs[0]), o1 = fmaf((float)a[q].y * xs, ws[1], bs[1]);
+      const float o2 = fmaf((float)a[q].z * xs, ws[2], bs[2]), o3 = fmaf((float)a[q].w * xs, ws[3], bs[3]);
+      const uint32_t lo = pack2(o0, o1, p.fp16), hi = pack2(o2, o3, p.fp16);
+      uint16_t* dst = static_cast<uint16_t*>(p.y) + (int64_t)(t0 + c) * p.N + n;
+      if ((p.N & 3) == 0) {
+        if (n < p.N) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+      } else {
+        if (n < p.N) dst[0] = (uint16_t)lo;
+        if (n + 1 < p.N) dst[1] = (uint16_t)(lo >> 16);
+        if (n + 2 < p.N) dst[2] = (uint16_t)hi;
+        if (n + 3 < p.N) dst[3] = (uint16_t)(hi >> 16);
+      }
     }
   }
   if (threadIdx.x == 0 && ctl->abort_word != 0 && p.status != nullptr) {
@@ -669,17 +679,16 @@ Variant pick_variant(int T, int N, int K, int force, bool quantise) {
   v.splits = 1;
   while (v.splits < 8 && tiles * v.splits * 2 <= 3 * sms && KB / (v.splits * 2) >= 2) v.splits *= 2;
   const int kb = (KB + v.splits - 1) / v.splits;
-  // Every CTA reads all rows: 64 KB at most, against the 16 KB of weights of each of its k-blocks.
-  v.fused = quantise && T <= kFusedTokens && (int64_t)T * KB * kTileKI8 <= 32768 && kb <= kFusedBlocks;
+  v.fused = quantise && T == 1 && kb <= kFusedBlocks;
   const int stage = kRowTileBytes + (v.fused ? 0 : v.tokens * kTileKI8);
-  v.stages = std::min({kb, kMaxStagesI8, 110 * 1024 / stage});
+  v.stages = std::min({kb, kMaxStagesI8, (110 * 1024 - (v.fused ? kb * kFusedBlockBytes : 0)) / stage});      // two CTAs to an SM
   return v;
 }
 
 }  // namespace
 
 struct LinearArgs {
-  const void* x; int64_t x_stride; int x_dtype;        // rows; int8 ones with q = x and their scale
+  const void* x; int x_dtype;                          // rows; int8 ones with q = x and their scale
   const void* q; const float* x_scale;
   const void* w; const float* w_scale; const float* bias;
   void* y;
@@ -696,9 +705,8 @@ int launch_linear_int8(const LinearArgs& a, const Variant& v, cudaStream_t st) {
   p.T = T; p.N = N; p.x_scale = a.x_scale; p.w_scale = a.w_scale; p.bias = a.bias; p.y = a.y; p.status = a.status; p.fp16 = a.fp16;
   if (!v.pair) {
     p.tokens = v.tokens; p.splits = v.splits; p.stages = v.stages; p.early_weights = a.early_weights;
-    p.x = a.x; p.x_stride = a.x_stride; p.x_dtype = a.x_dtype;
-    const int64_t row = 16 / (a.x_dtype == B200MOE_T_FP32 ? 4 : 2);
-    p.x_vec = ((uintptr_t)a.x & 15) == 0 && a.x_stride % row == 0;
+    p.x = a.x; p.x_dtype = a.x_dtype;
+    p.x_vec = ((uintptr_t)a.x & 15) == 0;
     if (!v.fused)
       if (int rc = encode_rows(&p.tmX, a.q, K, T, v.tokens, "int8 token rows")) return rc;
     if (int rc = encode_rows(&p.tmW, a.w, K, N, kRowTile, "int8 weights")) return rc;
@@ -769,7 +777,7 @@ extern "C" int b200moe_linear_int8(const void* x, int64_t x_stride, int32_t x_dt
   cudaStream_t st = (cudaStream_t)stream;
   const bool quantise = x_dtype != B200MOE_T_INT8;
   const Variant v = pick_variant(T, N, K, variant, quantise);
-  LinearArgs a = {x, x_stride, x_dtype, x, x_scale, weight, weight_scale, bias, y, T, N, K, out_dtype == B200MOE_T_FP16, quantise, status};
+  LinearArgs a = {x, x_dtype, x, x_scale, weight, weight_scale, bias, y, T, N, K, out_dtype == B200MOE_T_FP16, quantise, status};
   if (!quantise) {
     B200_CHECK_ARG(x_scale != nullptr && x_stride == K && ((uintptr_t)x & 15) == 0, "linear_int8: 8-bit rows must be contiguous, 16-byte aligned and have x_scale");
   } else {

@@ -111,7 +111,7 @@ def test_layer_matches_64_bits(T, N, K, variant):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("T,N,K", [(1, 2880, 2880), (1, 129, 16384), (8, 300, 4096), (3, 2880, 2896), (5, 14336, 2048), (8, 64, 16), (9, 64, 4096), (2, 40, 8208)])
 def test_few_tokens(T, N, K, dtype):
-    """The sizes around those that the split kernel quantises itself: rows on and off the 16-byte grid, apart from one another,
+    """One token, which the split kernel quantises itself, and a few: rows on and off the 16-byte grid, apart from one another,
     the last ones of a buffer."""
     g = torch.Generator().manual_seed(T * K)
     w, ws = _weight(N, K, T)
