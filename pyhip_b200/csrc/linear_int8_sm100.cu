@@ -714,9 +714,10 @@ int launch_linear_int8(const LinearArgs& a, const Variant& v, cudaStream_t st) {
     B200_CHECK_ARG(t_tiles <= 65535, "linear_int8: %d tokens", T);
     const int stage = kRowTileBytes + (v.fused ? 0 : v.tokens * kTileKI8);
     const int blocks = v.fused ? ((p.KB + v.splits - 1) / v.splits) * kFusedBlockBytes : 0;
-    // At least the share of shared memory that its columns are of tensor memory: CTAs that fit an SM's shared memory
-    // then fit its tensor memory too, and no cluster waits for columns that another waiting cluster holds.
-    const int share = (int)((int64_t)kSmemLimitI8 * std::max(32, v.tokens) / 512);
+    // At least the share of shared memory that its columns are of tensor memory: CTAs of this kernel that fit an SM's shared
+    // memory then fit its tensor memory too, and no cluster waits for columns that another waiting cluster holds.  And 64 KB
+    // at least, which leaves no room beside a kernel that takes all columns (those hold most of the shared memory).
+    const int share = std::max((int)((int64_t)kSmemLimitI8 * std::max(32, v.tokens) / 512), 64 * 1024);
     const int bytes = std::max({v.stages * stage + blocks, std::min(v.tokens, T) * kRowTile * 4 + 16 * kRowTile * 4, share});
     const size_t smem = 1024 + kCtlBytes + (size_t)bytes;
     void (*k)(LinearParams) = v.fused ? linear_int8_split_kernel<true> : linear_int8_split_kernel<false>;

@@ -183,6 +183,20 @@ def test_rows_that_hold_infinities_stay_their_own():
         assert torch.equal(y[keep], good[keep]) and y[~keep].isnan().all()
 
 
+def test_one_row_of_zeros_infinities_and_tiny_values():
+    w, ws = _weight(40, 128, 6)
+    x = torch.randn(1, 128, device=DEV, dtype=torch.float32)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        zero = torch.zeros(1, 128, device=DEV, dtype=dtype)
+        assert (linear_int8(zero, w, ws, out_dtype=torch.bfloat16) == 0).all()
+        for bad in (float("inf"), float("nan"), float("-inf")):
+            y = x.to(dtype)
+            y[0, 77] = bad
+            assert linear_int8(y, w, ws, out_dtype=torch.bfloat16).isnan().all()
+        tiny = (x * 1e-6).to(dtype)
+        _check(linear_int8(tiny, w, ws, out_dtype=torch.bfloat16), *orc.linear_int8(*orc.quantize_int8(tiny), w, ws))
+
+
 @pytest.mark.parametrize("T", [3, 900])
 def test_rows_behind_the_output_are_left_alone(T):
     """The output's neighbours in memory: a layer call must not write outside its rows, whichever way they are stored."""
