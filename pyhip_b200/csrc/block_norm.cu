@@ -7,9 +7,13 @@
 // Bound by memory: forward reads y and r and writes h and n (8 bytes a value in 16-bit types), backward reads
 // y, r, dh, dn and writes dy and dr (12 bytes).  The threads that share a row take the same columns of every row, in
 // 16-byte pieces, so every value is read and written once and the sums over tokens stay in registers.
-// Two forms.  Plain: a row goes straight to registers; any alignment, and the lowest latency for few rows.  Ring: a
+// Two forms.  Plain: a row goes straight to registers; any alignment, and the better one for narrow rows.  Ring: a
 // thread copies its pieces of the next rows to shared memory while it works on the present one (it reads nothing but
 // its own copies, so no barrier), which keeps tens of KB in flight per SM where the plain form waits at every row.
+// On a B200 (6.55 TB/s measured): forward 8192 x 2880 33 us, 5.7 TB/s; 8192 x 4096 43 us, 6.2 TB/s; 4096 x 7168 45 us,
+// 5.3 TB/s.  Backward 4096 x 7168 80 us, 4.4 TB/s; 8192 x 4096 80-84 us, 4.8 TB/s; 16384 x 2048 83 us, 4.8 TB/s: the three
+// sums of a row end in a barrier that a CTA's warps reach together.  Quantiser 16384 x 4096 48 us, 4.1 TB/s: a row's reduction
+// and scale cost each warp as much as 9 of its values.
 #include <algorithm>
 
 #include "rowwise.cuh"
@@ -705,17 +709,19 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
   }
 }
 
-// dst[c] = sum over the partial rows, in ascending order within eight interleaved groups that are then added in order.
+// dst[c] = sum over the partial rows, in ascending order within 32 interleaved groups that are then added in order.  The
+// groups are many because the columns are few: with 8 of them this was most of a backward pass over narrow rows.
 struct ColumnSumParams {
   const float* part;
   void* dst[3];
   int f32[3];
   int rows, H;
 };
+constexpr int kSumGroups = 32;
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kSumGroups * 32)
 column_sum_kernel(const __grid_constant__ ColumnSumParams p) {
-  __shared__ float s[8][33];
+  __shared__ float s[kSumGroups][33];
   grid_dep_wait();
   grid_dep_launch();
   const int which = blockIdx.y, col = blockIdx.x * 32 + (threadIdx.x & 31), grp = threadIdx.x >> 5;
@@ -723,13 +729,13 @@ column_sum_kernel(const __grid_constant__ ColumnSumParams p) {
   float a = 0.f;
   if (col < p.H)
 #pragma unroll 8
-    for (int r = grp; r < p.rows; r += 8) a += p.part[((int64_t)r * 3 + which) * p.H + col];
+    for (int r = grp; r < p.rows; r += kSumGroups) a += p.part[((int64_t)r * 3 + which) * p.H + col];
   s[grp][threadIdx.x & 31] = a;
   __syncthreads();
   if (grp == 0 && col < p.H) {
     float v[1] = {0.f};
 #pragma unroll
-    for (int g = 0; g < 8; ++g) v[0] += s[g][threadIdx.x];
+    for (int g = 0; g < kSumGroups; ++g) v[0] += s[g][threadIdx.x];
     store_param<T, 1>(p.dst[which], p.f32[which], col, v);
   }
 }
@@ -758,11 +764,13 @@ bool vector_ok(const NormParams& p) {
          (p.gate_kind == B200MOE_GATE_TOKEN || aligned16(p.gate)) && aligned16(p.wn) && aligned16(p.h) && aligned16(p.n) && aligned16(p.q);
 }
 
-// The ring needs its gate rows in the rows' type, its weights in one type, a width that gives whole warps something to do,
-// and more rows than the SMs take at once.
+// The ring needs its gate rows in the rows' type, its weights in one type, and a width that gives its warps something to do.
+// Plain against ring, us (bf16 with a residual and both norms; forward, backward):  4096 x 256: 3.4, 19.0 against 4.3, 17.6;
+// 4096 x 512: 6.1, 23.9 against 4.7, 21.3;  128 x 512: 2.7, 7.4 against 2.6, 5.7;  64 x 2880: 2.9, 9.2 against 2.8, 8.6;
+// 4096 x 2880: 40.0, 73.2 against 16.9, 41.2.
 template <typename T>
 bool ring_ok(const NormParams& p, bool vec) {
-  return vec && p.H >= 512 && p.T >= 4 * device_sm_count() && (sizeof(T) == 4 || p.w == nullptr || p.wn == nullptr || p.w_f32 == p.wn_f32) &&
+  return vec && p.H >= 512 && (sizeof(T) == 4 || p.w == nullptr || p.wn == nullptr || p.w_f32 == p.wn_f32) &&
          (p.gate_kind != B200MOE_GATE_FULL || sizeof(T) == 4 || !p.gate_f32);
 }
 // whether the weights are fp32 (they are of one type)
@@ -890,7 +898,7 @@ int launch_norm_bwd_t(const NormBwdParams& b, const ColumnSumParams& sums, cudaS
     c.part = b.part;
     c.rows = r.grid * r.s.rows;
     c.H = p.H;
-    B200_CHECK_CUDA(launch_chained(column_sum_kernel<T>, dim3((p.H + 31) / 32, 3), dim3(256), 0, st, c));
+    B200_CHECK_CUDA(launch_chained(column_sum_kernel<T>, dim3((p.H + 31) / 32, 3), dim3(kSumGroups * 32), 0, st, c));
   }
   return 0;
 }

@@ -12,6 +12,11 @@
 //   pair    persistent CTA pairs (cta_group::2), 256 tokens x BN features a tile: each CTA holds its 128 tokens' rows and
 //           half of the feature rows, two accumulators overlap a tile's epilogue with the next one's products.
 //
+// On a B200 (tokens, weight N x K): 1, 2880 x 2880 6.2-6.6 us; 64, 14336 x 4096 15.4 us (17.3 with the quantiser; the weights'
+// stream alone is 9); 64, 4096 x 4096 10 us; 512, 4096 x 4096 12.9 us; 1000, 2048 x 7168 17.6 us; 2048, 7168 x 4096 43 us;
+// 16384, 14336 x 4096 590 us, 3.26 POP/s, tensor pipe 89 % active.  What a call does not overlap, 6 to 7 us, bounds the small
+// ones: start and first load 2, the last tile's way out and the join 3 to 4.
+//
 // A pipeline stage is 128 bytes of K (one swizzle span): 128 rows of one operand and BT or BN/2 rows of the other, one TMA
 // copy each; K and row tails are zero-filled by the copy.  Every barrier wait is bounded; one that runs out sets status[]
 // and the CTA unwinds and frees its tensor memory.

@@ -13,6 +13,9 @@
 // consecutive rows.  Sums over tokens: a chunk and a sequence that overlap write one row of partial sums at slot
 // chunk + sequence -- the overlapping pairs form a staircase, so no two share a slot -- and a second launch adds the
 // slots of a sequence in order.  No atomics on floats: the same bits on every run.
+// On a B200: 64 x 128 experts, top 4: 3.7 + 4.1 us; 16384 x 8, top 2: 4.7 + 6.9, backward 3.4 us; 4096 x 256, top 8: 10.1 + 7.3,
+// backward 8.4 us, with sigmoid scores, a mask and 13 sequences 16.0 + 6.1 and 10.4 us; 16384 x 256: 29 + 8.6, 17.7 us (the
+// selection's instructions).  A launch with a single row takes 5 us.
 #include <algorithm>
 
 #include "rowwise.cuh"

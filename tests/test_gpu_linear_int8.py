@@ -190,7 +190,7 @@ def test_one_row_of_zeros_infinities_and_tiny_values():
         zero = torch.zeros(1, 128, device=DEV, dtype=dtype)
         assert (linear_int8(zero, w, ws, out_dtype=torch.bfloat16) == 0).all()
         for bad in (float("inf"), float("nan"), float("-inf")):
-            y = x.to(dtype)
+            y = x.to(dtype).clone()
             y[0, 77] = bad
             assert linear_int8(y, w, ws, out_dtype=torch.bfloat16).isnan().all()
         tiny = (x * 1e-6).to(dtype)

@@ -215,7 +215,10 @@ def test_int8_rows(T, H, dtype):
     one = torch.ones(H, device=DEV)
     q2, s2 = fused_pre_norm(x, one, quant="int8")
     q3, s3, h3 = fused_pre_norm(x, one, residual=torch.zeros_like(x), quant="int8")
-    assert torch.equal(q2, q3) and torch.equal(s2, s3) and torch.equal(h3, x)
+    # a row whose copies with the residual do not fit the ring adds its squares in another order: both sides' largest value is
+    # within C of the exact one (and a rounding more in the division), so the scales within twice that of one another, and a
+    # quotient of at most 127 moves by less than 127 * 2 * C < 0.01, one step of the grid at most
+    assert ((s2 - s3).abs() <= 2 * (C + 2.0 ** -23) * s2).all() and (q2.int() - q3.int()).abs().max() <= 1 and torch.equal(h3, x)
     qq, ss = quantize_int8(x)
     assert (q2.int() - qq.int()).abs().max() <= 1
 
