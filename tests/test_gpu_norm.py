@@ -94,6 +94,28 @@ def test_backward_matches_64_bits(T, H, dtype):
             _near(got[name], *want[name], f"{name} (case {k})")
 
 
+@pytest.mark.parametrize("T,H", [(5, 96), (300, 2880), (40, 7168), (3, 16384)])
+@pytest.mark.parametrize("gate", ["channel", "token", "full"])
+def test_parameters_of_different_types(T, H, gate):
+    """Weights, next weights and gates each fp32 or of the rows' type."""
+    bf, f = torch.bfloat16, torch.float32
+    for k, (wt, gt, nt) in enumerate([(f, bf, bf), (bf, bf, f), (bf, f, bf), (f, f, bf), (f, bf, f)]):
+        i = _inputs(T, H, bf, f, True, gate, True, seed=T + k)
+        i = dict(i, weight=i["weight"].to(wt), gate=i["gate"].to(gt), next_weight=i["next_weight"].to(nt))
+        o = orc.block_norm(i["y"], i["residual"], i["weight"], i["gate"], 0.75, 1e-5, i["next_weight"])
+        for t in i.values():
+            t.requires_grad_(True)
+        dh, dn = _randn(T, H, seed=k, dtype=bf), _randn(T, H, seed=k + 50, dtype=bf)
+        r = fused_post_norm(i["y"], i["residual"], i["weight"], gate=i["gate"], residual_scale=0.75, eps=1e-5, next_weight=i["next_weight"])
+        _near(r[0].detach(), o["h"], o["h_size"], "h")
+        _near(r[1].detach(), o["n"], o["n_size"], "n")
+        got = _grads(i, r, dh, dn)
+        want = orc.block_norm_grads(o, i["residual"], i["weight"], i["gate"], 0.75, i["next_weight"], dh, dn)
+        for name in want:
+            assert got[name].dtype == i[name].dtype
+            _near(got[name], want[name][0].detach(), want[name][1].detach(), f"{name} (case {k})")
+
+
 def test_formula_matches_differences():
     """The oracle's gradients (64 bits) against central differences of its forward."""
     i = {k: None if v is None else v.double().cpu() for k, v in _inputs(3, 5, torch.float32, torch.float32, True, "token", True).items()}
