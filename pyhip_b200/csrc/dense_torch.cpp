@@ -6,11 +6,14 @@
 // Python backward node another 40 to 80 us on top of autograd's own 40.  Here a call costs little more than its launches.
 #include <torch/extension.h>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
+#include <initializer_list>
 #include <mutex>
 #include <optional>
 #include <string>
@@ -50,6 +53,24 @@ void need_cuda(const Tensor& x, const char* what) {
 void need_no_grad(bool requires_grad, const char* what) {
   if (requires_grad && at::GradMode::is_enabled())
     throw std::runtime_error(std::string(what) + ": call it under torch.no_grad() or on detached tensors");
+}
+// What torch may lay over a call and these kernels, which torch's dispatcher does not see, cannot take part in.  A dual tensor of
+// forward-mode differentiation does not require a gradient: it would come back without its tangent.  A trace would record the
+// empty outputs and none of the kernels that fill them.  `no_grad` ends neither.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+void need_no_tangent(bool any, const char* what) {
+  if (any && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    throw std::runtime_error(std::string(what) + " has no forward-mode derivative: unpack the dual tensors first");
+}
+void need_eager(const char* what) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  bool traced = torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+  if (TorchDispatchModeTLS::any_modes_set())
+    for (const auto mode : {TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FAKE, TorchDispatchModeKey::FUNCTIONAL})
+      traced = traced || TorchDispatchModeTLS::get_mode(mode).has_value();
+  if (traced) throw std::runtime_error(std::string(what) + " runs its own kernels and cannot be traced: call it outside of the traced function");
 }
 
 int row_type(at::ScalarType t) {
@@ -92,6 +113,8 @@ int32_t as_i32(int64_t v, const char* what) {
 // ------------------------------------------------------------------------------------ 8-bit integers
 std::tuple<Tensor, Tensor> quantize_int8(const Tensor& x) {
   need_cuda(x, "quantize_int8");
+  need_eager("quantize_int8");
+  need_no_tangent(has_tangent(x), "quantize_int8");
   const int dt = row_type(x.scalar_type());
   TYPE_CHECK(dt >= 0, "x must be bfloat16, float16 or float32");
   VALUE_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= kMaxRow, "rows of x must have 1 to ", kMaxRow, " values");
@@ -133,6 +156,8 @@ OptTensor int8_status(int64_t device) {
 Tensor linear_int8(const Tensor& x, const Tensor& weight, const Tensor& weight_scale, const OptTensor& x_scale, const OptTensor& bias,
                    std::optional<at::ScalarType> out_dtype, int64_t variant) {
   need_cuda(x, "linear_int8");
+  need_eager("linear_int8");
+  need_no_tangent(has_tangent(x) || has_tangent(weight_scale) || has_tangent(x_scale) || has_tangent(bias), "linear_int8");
   TYPE_CHECK(weight.scalar_type() == at::kChar && weight.dim() == 2, "weight must be an int8 matrix [N, K]");
   const int64_t N = weight.size(0), K = weight.size(1);
   VALUE_CHECK(x.dim() >= 1 && x.size(-1) == K, "x has shape ", x.sizes(), ", the weight ", K, " columns");
@@ -225,6 +250,13 @@ NormOutputs norm_forward(const Tensor& y, const OptTensor& residual, const OptTe
   return o;
 }
 
+void need_first_order(const variable_list& up, const char* what) {
+  need_eager(what);
+  bool any = false;
+  for (const Tensor& g : up) any = any || has_tangent(g);
+  need_no_tangent(any, what);
+}
+
 // Gradients of a backward pass that is itself being recorded: nothing here can be differentiated again, and says so.
 variable_list once(variable_list grads, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -248,6 +280,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list up) {
+    need_first_order(up, "the block norm's backward pass");
     const auto s = ctx->get_saved_variables();
     const auto [kind, alpha, want_h] = ctx->saved_data["how"].to<std::tuple<int64_t, double, bool>>();
     const Tensor& y = s[0];
@@ -283,6 +316,8 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
 variable_list block_norm(const Tensor& y, const OptTensor& residual, const OptTensor& weight, const OptTensor& gate, const OptTensor& next,
                          double alpha, double eps, bool want_h, bool quant, const std::string& what) {
   need_cuda(y, what.c_str());
+  need_eager(what.c_str());
+  need_no_tangent(has_tangent(y) || has_tangent(residual) || has_tangent(weight) || has_tangent(gate) || has_tangent(next), what.c_str());
   const auto dtype = y.scalar_type();
   TYPE_CHECK(row_type(dtype) >= 0, "rows must be bfloat16, float16 or float32");
   const int64_t H = y.dim() ? y.size(-1) : 0;
@@ -373,6 +408,7 @@ struct Router : torch::autograd::Function<Router> {
     return r.out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list up) {
+    need_first_order(up, "fused_router's backward pass");
     const auto s = ctx->get_saved_variables();
     const auto [K, scoring, renorm, S] = ctx->saved_data["how"].to<std::tuple<int64_t, int64_t, bool, int64_t>>();
     const Tensor& logits = s[0];
@@ -395,6 +431,8 @@ struct Router : torch::autograd::Function<Router> {
 
 variable_list router(const Tensor& logits, int64_t K, bool renorm, const std::string& scoring, const OptTensor& mask, const OptTensor& cu) {
   need_cuda(logits, "fused_router");
+  need_eager("fused_router");
+  need_no_tangent(has_tangent(logits), "fused_router");
   TYPE_CHECK(row_type(logits.scalar_type()) >= 0, "gating_output must be bfloat16, float16 or float32");
   VALUE_CHECK(logits.dim() == 2, "gating_output must be [T, E]");
   const int64_t T = logits.size(0), E = logits.size(1);

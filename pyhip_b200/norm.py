@@ -15,7 +15,7 @@ def fused_pre_norm(x, weight, *, residual=None, eps=1e-6, quant=None):
       ``weight``: [H], of the rows' type or float32
       ``quant="int8"``: n as 8-bit integers with one scale per token, for `linear_int8`; no gradient
 
-    Arithmetic in 32 bits, each result rounded once; n is the norm of the unrounded sum.
+    Arithmetic in 32 bits, each result rounded once; n is the norm of the unrounded sum.  Differentiable as `fused_post_norm`.
     Returns n, or (q, scale) with ``quant``; with ``residual`` followed by h, the new residual stream."""
     if weight is None:
         raise ValueError("fused_pre_norm needs a weight")
@@ -35,8 +35,9 @@ def fused_post_norm(y, residual, weight=None, *, gate=None, residual_scale=1.0, 
       ``gate``: [H] per channel, [..., 1] per token, or [..., H]; the rows' type or float32, as ``weight`` and ``next_weight`` [H]
       ``quant="int8"``: n as 8-bit integers with one scale per token, for `linear_int8`; no gradient
 
-    Arithmetic in 32 bits, each result rounded once; n is the norm of the unrounded h.  Differentiable in all five tensors;
-    gradients that sum over tokens are added in a fixed order.
+    Arithmetic in 32 bits, each result rounded once; n is the norm of the unrounded h.  Differentiable in all five tensors, in
+    reverse mode and once; forward-mode derivatives and tracing are refused.  Gradients that sum over tokens are added in a fixed
+    order.
     Returns h; (h, n) with ``next_weight``; (h, q, scale) with ``quant`` as well."""
     if residual is None:
         raise ValueError("fused_post_norm needs the residual")

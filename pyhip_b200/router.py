@@ -22,7 +22,8 @@ class RouterOutput(NamedTuple):
 
 def fused_router(gating_output, topk: int, *, renormalize: bool = True, scoring: str = "softmax", token_mask=None,
                  cu_seqlens=None) -> RouterOutput:
-    """Top-k routing with per-expert counts, balance loss and z-loss, differentiable in the logits.
+    """Top-k routing with per-expert counts, balance loss and z-loss, differentiable in the logits (in reverse mode and once;
+    forward-mode derivatives and tracing are refused).
 
       ``gating_output``: logits [T, E], bf16, fp16 or fp32, E <= 1024; rows may lie apart
       ``topk``: experts per token, up to 32; the largest LOGITS, equal ones in ascending order

@@ -1,0 +1,85 @@
+"""GPU tier: the dense operators under what torch lays over a call -- forward-mode derivatives and tracing.  Where an
+operator cannot take part it has to say so: a result without its tangent or a trace without the kernel is a wrong answer."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+from pyhip_b200 import fused_post_norm, fused_pre_norm, fused_router, linear_int8, quantize_int8
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _tensors():
+    g = torch.Generator().manual_seed(3)
+    t = dict(x=torch.randn(6, 64, generator=g), r=torch.randn(6, 64, generator=g), w=torch.randn(64, generator=g) + 2, g=torch.randn(6, 1, generator=g),
+             n=torch.randn(64, generator=g) + 2, logits=torch.randn(6, 16, generator=g), ws=torch.rand(32, generator=g) + 0.1, b=torch.randn(32, generator=g))
+    t = {k: v.to(DEV) for k, v in t.items()}
+    t["q"], t["qs"] = quantize_int8(t["x"])
+    t["iw"] = torch.randint(-127, 128, (32, 64), generator=g, dtype=torch.int8).to(DEV)
+    t["mask"] = torch.tensor([True, True, False, True, True, True], device=DEV)
+    t["cu"] = torch.tensor([0, 2, 5], dtype=torch.int32, device=DEV)
+    return t
+
+
+# every call with the names of the float tensors that it takes
+CALLS = {
+    "pre_norm": (lambda t: fused_pre_norm(t["x"], t["w"], residual=t["r"]), "x w r"),
+    "pre_norm_int8": (lambda t: fused_pre_norm(t["x"], t["w"], residual=t["r"], quant="int8"), "x w r"),
+    "post_norm": (lambda t: fused_post_norm(t["x"], t["r"], t["w"], gate=t["g"], next_weight=t["n"]), "x r w g n"),
+    "router": (lambda t: fused_router(t["logits"], 3, token_mask=t["mask"], cu_seqlens=t["cu"]), "logits"),
+    "quantize": (lambda t: quantize_int8(t["x"]), "x"),
+    "linear": (lambda t: linear_int8(t["x"], t["iw"], t["ws"], bias=t["b"]), "x ws b"),
+    "linear_int8_rows": (lambda t: linear_int8(t["q"], t["iw"], t["ws"], x_scale=t["qs"]), "ws qs"),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_forward_mode_is_refused(name):
+    call, names = CALLS[name]
+    t = _tensors()
+    for key in names.split():
+        with fw.dual_level():
+            d = dict(t, **{key: fw.make_dual(t[key], torch.ones_like(t[key]))})
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(d)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):      # forward mode goes on there
+                call(d)
+        call(t)
+
+
+def test_forward_mode_over_the_backward_pass_is_refused():
+    t = _tensors()
+    for call, leaf in ((lambda x: fused_pre_norm(x, t["w"]), t["x"]), (lambda x: fused_router(x, 3).topk_weights, t["logits"])):
+        x = leaf.clone().requires_grad_(True)
+        out = call(x)
+        with fw.dual_level():
+            up = fw.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, x, up)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_tracing_is_refused(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, names = CALLS[name]
+    t = _tensors()
+    key = names.split()[0]
+
+    def f(v):
+        return tuple(call(dict(t, **{key: v}))) if name != "linear" and name != "linear_int8_rows" else call(dict(t, **{key: v}))
+
+    with torch.no_grad():
+        for trace in (lambda: torch.jit.trace(f, (t[key],), check_trace=False), lambda: make_fx(f)(t[key]), lambda: make_fx(f, pre_dispatch=True)(t[key])):
+            with pytest.raises(RuntimeError, match="trac"):
+                trace()
+
+
+def test_tracing_the_backward_pass_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    t = _tensors()
+    for call, leaf in ((lambda x: fused_pre_norm(x, t["w"]), t["x"]), (lambda x: fused_router(x, 3).topk_weights, t["logits"])):
+        x = leaf.clone().requires_grad_(True)
+        out = call(x)
+        with pytest.raises(RuntimeError, match="trac"):
+            make_fx(lambda up: torch.autograd.grad(out, x, up))(torch.ones_like(out))
