@@ -81,7 +81,14 @@ int row_type(at::ScalarType t) {
     default: return -1;
   }
 }
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// Null means an absent tensor to the C calls, so one that is there must not come as null: a wrapper around another tensor (a subclass
+// without memory of its own) would be taken for none.
+void* ptr(const Tensor& t) {
+  if (!t.defined()) return nullptr;
+  void* p = t.data_ptr();
+  TYPE_CHECK(p != nullptr || t.numel() == 0, "a tensor of shape ", t.sizes(), " has no memory of its own: pass the tensor that it wraps");
+  return p;
+}
 void* ptr(const OptTensor& t) { return t.has_value() ? ptr(*t) : nullptr; }
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 bool on(const OptTensor& t, const Tensor& like) { return !t.has_value() || t->device() == like.device(); }
@@ -105,6 +112,8 @@ Rows rows_of(const Tensor& x) {
   r.stride = r.T > 1 ? r.t.stride(0) : r.H;
   return r;
 }
+// an upstream gradient as the kernels read it; one that is known to be zero has no memory and counts for none
+Tensor upstream(const Tensor& g) { return g.defined() && !g._is_zerotensor() ? g.contiguous() : Tensor(); }
 int32_t as_i32(int64_t v, const char* what) {
   VALUE_CHECK(v < (int64_t(1) << 31), what, " is too large: ", v);
   return (int32_t)v;
@@ -290,9 +299,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
       at::NoGradGuard no_grad;
       c10::cuda::CUDAGuard guard(y.device());
       const NormInputs i(y, opt(1), opt(2), opt(3), opt(4), (int32_t)kind);
-      Tensor dh = want_h ? up[0] : Tensor(), dn = s[4].defined() ? up[want_h ? 1 : 0] : Tensor();
-      if (dh.defined()) dh = dh.contiguous();
-      if (dn.defined()) dn = dn.contiguous();
+      const Tensor dh = want_h ? upstream(up[0]) : Tensor(), dn = s[4].defined() ? upstream(up[want_h ? 1 : 0]) : Tensor();
       size_t edge = 0;                       // edges are numbered over the tensors that are there
       for (int k = 0; k < 5; ++k)
         if (s[k].defined() && ctx->needs_input_grad(edge++)) grads[k] = empty_as(s[k], s[k].sizes(), s[k].scalar_type());
@@ -418,11 +425,11 @@ struct Router : torch::autograd::Function<Router> {
       c10::cuda::CUDAGuard guard(logits.device());
       const Rows x = rows_of(logits);
       const Saved k(s[3], x.T, S, x.H);
-      const Tensor dw = up[0].defined() ? up[0].contiguous() : Tensor();
+      const Tensor dw = upstream(up[0]), db = upstream(up[3]), dz = upstream(up[4]);
       grads[0] = empty_as(logits, logits.sizes(), logits.scalar_type());
       call_check(b200moe_router_backward(ptr(x.t), x.stride, (int32_t)x.T, (int32_t)x.H, (int32_t)K, row_type(logits.scalar_type()),
                                          (int32_t)scoring, renorm, k.lse, k.seg, k.coef, k.stats, s[2].data_ptr<int32_t>(),
-                                         s[1].data_ptr<float>(), (const float*)ptr(dw), (const float*)ptr(up[3]), (const float*)ptr(up[4]),
+                                         s[1].data_ptr<float>(), (const float*)ptr(dw), (const float*)ptr(db), (const float*)ptr(dz),
                                          ptr(grads[0]), stream_of(logits)), "router_backward");
     }
     return once(std::move(grads), "fused_router");

@@ -1,4 +1,4 @@
-"""GPU tier: the dense operators under what torch lays over a call -- forward-mode derivatives and tracing.  Where an
+"""GPU tier: the dense operators under what torch lays over a call -- forward-mode derivatives, tracing, wrapped tensors.  Where an
 operator cannot take part it has to say so: a result without its tangent or a trace without the kernel is a wrong answer."""
 import pytest
 import torch
@@ -83,3 +83,55 @@ def test_tracing_the_backward_pass_is_refused():
         out = call(x)
         with pytest.raises(RuntimeError, match="trac"):
             make_fx(lambda up: torch.autograd.grad(out, x, up))(torch.ones_like(out))
+
+
+class Wrapped(torch.Tensor):
+    """A tensor that holds another one and has no memory of its own."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+    def __init__(self, t):
+        self.inner = t
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        return func(*(a.inner if isinstance(a, cls) else a for a in args), **(kwargs or {}))
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_wrapped_tensors_are_refused(name):
+    call, names = CALLS[name]
+    t = _tensors()
+    extra = dict(router=" mask cu", linear=" iw", linear_int8_rows=" q iw").get(name, "")
+    for key in (names + extra).split():
+        with torch.no_grad(), pytest.raises((TypeError, RuntimeError)):
+            call(dict(t, **{key: Wrapped(t[key])}))
+    with torch.no_grad(), pytest.raises((TypeError, RuntimeError)):
+        torch.func.vmap(lambda v: call(dict(t, **{names.split()[-1]: v})))(torch.stack([t[names.split()[-1]]] * 2))
+
+
+def test_batched_gradients_are_refused():
+    t = _tensors()
+    x = t["x"].clone().requires_grad_(True)
+    out = fused_pre_norm(x, t["w"])
+    with pytest.raises((TypeError, RuntimeError)):
+        torch.autograd.grad(out, x, torch.ones(3, *out.shape, device=DEV), is_grads_batched=True)
+
+
+def test_upstream_gradients_that_are_known_to_be_zero():
+    t = _tensors()
+    x, w = t["x"].clone().requires_grad_(True), t["w"].clone().requires_grad_(True)
+    n, h = fused_pre_norm(x, w, residual=t["r"])
+    zero = torch._efficientzerotensor(n.shape, dtype=n.dtype, device=n.device)
+    got = torch.autograd.grad([n, h], [x, w], [zero, torch.ones_like(h)], retain_graph=True)
+    want = torch.autograd.grad([n, h], [x, w], [torch.zeros_like(n), torch.ones_like(h)])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_sparse_tensors_are_refused():
+    t = _tensors()
+    for key in ("x", "w"):
+        with pytest.raises((TypeError, RuntimeError)):
+            fused_pre_norm(**{"x": t["x"], "weight": t["w"], {"x": "x", "w": "weight"}[key]: t[key].to_sparse()})
