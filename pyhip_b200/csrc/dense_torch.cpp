@@ -95,12 +95,17 @@ bool on(const OptTensor& t, const Tensor& like) { return !t.has_value() || t->de
 bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 Tensor empty_as(const Tensor& t, at::IntArrayRef shape, at::ScalarType dtype) { return at::empty(shape, t.options().dtype(dtype).requires_grad(false)); }
 
+// The values as memory holds them: a negation that torch has put off (a view of a conjugate's imaginary part) is made first.
+Tensor settled(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor packed(const Tensor& t) { return settled(t).contiguous(); }
+
 // [..., H] as T rows of H neighbouring values, `stride` elements apart; a view wherever one exists
 struct Rows {
   Tensor t;
   int64_t T, H, stride;
 };
-Rows rows_of(const Tensor& x) {
+Rows rows_of(const Tensor& as_given) {
+  const Tensor x = settled(as_given);
   Rows r{x, 0, x.size(-1), 0};
   r.T = r.H ? x.numel() / r.H : 0;
   if (x.is_contiguous()) {
@@ -113,7 +118,7 @@ Rows rows_of(const Tensor& x) {
   return r;
 }
 // an upstream gradient as the kernels read it; one that is known to be zero has no memory and counts for none
-Tensor upstream(const Tensor& g) { return g.defined() && !g._is_zerotensor() ? g.contiguous() : Tensor(); }
+Tensor upstream(const Tensor& g) { return g.defined() && !g._is_zerotensor() ? packed(g) : Tensor(); }
 int32_t as_i32(int64_t v, const char* what) {
   VALUE_CHECK(v < (int64_t(1) << 31), what, " is too large: ", v);
   return (int32_t)v;
@@ -203,13 +208,14 @@ Tensor linear_int8(const Tensor& x, const Tensor& weight, const Tensor& weight_s
       r.t = r.t.clone(at::MemoryFormat::Contiguous);
       r.stride = K;
     }
-    xs = x_scale->contiguous();
+    xs = packed(*x_scale);
   } else {
     call_check(b200moe_linear_int8_workspace(T, n, (int32_t)K, (int32_t)variant, &bytes), "linear_int8_workspace");
     if (bytes) ws = empty_as(x, {bytes}, at::kByte);
   }
-  const Tensor w = weight.is_contiguous() && ((uintptr_t)ptr(weight) & 15) == 0 ? weight : weight.clone(at::MemoryFormat::Contiguous);
-  const Tensor sc = weight_scale.contiguous(), b = bias ? bias->contiguous() : Tensor();
+  Tensor w = packed(weight);
+  if ((uintptr_t)ptr(w) & 15) w = w.clone();
+  const Tensor sc = packed(weight_scale), b = bias ? packed(*bias) : Tensor();
   call_check(b200moe_linear_int8(ptr(r.t), r.stride, dt, (const float*)ptr(xs), ptr(w), (const float*)ptr(sc), (const float*)ptr(b), T, n,
                                  (int32_t)K, row_type(out), (int32_t)variant, ptr(ws), bytes, status_of(x, stream), ptr(y), stream),
              "linear_int8");
@@ -226,10 +232,10 @@ struct NormInputs {
   NormInputs(const Tensor& y_, const OptTensor& residual, const OptTensor& weight, const OptTensor& gate, const OptTensor& next, int32_t kind_)
       : y(rows_of(y_)), r{}, g{}, kind(kind_), dt(row_type(y_.scalar_type())) {
     if (residual) r = rows_of(*residual);
-    if (weight) w = weight->contiguous();
-    if (next) wn = next->contiguous();
+    if (weight) w = packed(*weight);
+    if (next) wn = packed(*next);
     if (gate) {
-      if (kind == B200MOE_GATE_FULL) g = rows_of(*gate); else { g.t = gate->contiguous(); g.stride = 1; }
+      if (kind == B200MOE_GATE_FULL) g = rows_of(*gate); else { g.t = packed(*gate); g.stride = 1; }
     }
     bits = (w.defined() && w.scalar_type() == at::kFloat) | (gate && gate->scalar_type() == at::kFloat) << 1 |
            (wn.defined() && wn.scalar_type() == at::kFloat) << 2;
@@ -384,7 +390,7 @@ RouterResult router_forward(const Tensor& logits, int64_t K, int64_t scoring, bo
   const Rows x = rows_of(logits);
   const int64_t T = x.T, E = x.H, S = cu ? cu->size(0) - 1 : 1;
   as_i32(T, "the number of tokens"), as_i32(S, "the number of sequences");
-  const Tensor m = mask ? mask->contiguous() : Tensor(), c = cu ? cu->contiguous() : Tensor();
+  const Tensor m = mask ? packed(*mask) : Tensor(), c = cu ? packed(*cu) : Tensor();
   int64_t bytes = 0;
   call_check(b200moe_router_workspace((int32_t)T, (int32_t)E, (int32_t)S, &bytes), "router_workspace");
   RouterResult r;

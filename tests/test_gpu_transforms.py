@@ -1,5 +1,6 @@
-"""GPU tier: the dense operators under what torch lays over a call -- forward-mode derivatives, tracing, wrapped tensors.  Where an
-operator cannot take part it has to say so: a result without its tangent or a trace without the kernel is a wrong answer."""
+"""GPU tier: the dense operators under what torch lays over a call -- forward-mode derivatives, tracing, wrapped tensors, lazy
+negation.  Where an operator cannot take part it has to say so: a result without its tangent or a trace without the kernel is a
+wrong answer."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
@@ -135,3 +136,29 @@ def test_sparse_tensors_are_refused():
     for key in ("x", "w"):
         with pytest.raises((TypeError, RuntimeError)):
             fused_pre_norm(**{"x": t["x"], "weight": t["w"], {"x": "x", "w": "weight"}[key]: t[key].to_sparse()})
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_lazily_negated_tensors_are_read_as_such(name):
+    """The imaginary part of a conjugate is a view with a negation that is still to be made."""
+    call, names = CALLS[name]
+    t = _tensors()
+    for key in names.split():
+        for v in (torch.complex(torch.zeros_like(t[key]), -t[key]).conj().imag, torch._neg_view(-t[key])):      # strided and dense
+            assert v.is_neg() and torch.equal(v, t[key])
+            with torch.no_grad():
+                got, want = call(dict(t, **{key: v})), call(t)
+            for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+                assert torch.equal(a, b)
+
+
+def test_lazily_negated_gradients_are_read_as_such():
+    t = _tensors()
+    for call, leaf in ((lambda x: fused_pre_norm(x, t["w"]), t["x"]), (lambda x: fused_router(x, 3).topk_weights, t["logits"]),
+                       (lambda x: fused_router(x, 3).z_loss, t["logits"])):
+        x = leaf.clone().requires_grad_(True)
+        up = torch.randn_like(call(x))
+        want, = torch.autograd.grad(call(x), x, up)
+        for v in (torch.complex(torch.zeros_like(up), -up).conj().imag, torch._neg_view(-up)):
+            assert v.is_neg()
+            assert torch.equal(torch.autograd.grad(call(x), x, v)[0], want)
