@@ -162,3 +162,17 @@ def test_lazily_negated_gradients_are_read_as_such():
         for v in (torch.complex(torch.zeros_like(up), -up).conj().imag, torch._neg_view(-up)):
             assert v.is_neg()
             assert torch.equal(torch.autograd.grad(call(x), x, v)[0], want)
+
+
+def test_a_learned_residual_scale_is_refused():
+    """residual_scale is a number: a parameter in its place would train without a gradient."""
+    t = _tensors()
+    p = torch.nn.Parameter(torch.tensor(0.5, device=DEV))
+    with pytest.raises(RuntimeError, match="residual_scale"):
+        fused_post_norm(t["x"], t["r"], residual_scale=p)
+    with pytest.raises(RuntimeError, match="eps"):
+        fused_pre_norm(t["x"], t["w"], eps=p)
+    with fw.dual_level(), pytest.raises(RuntimeError, match="residual_scale"):
+        fused_post_norm(t["x"], t["r"], residual_scale=fw.make_dual(torch.tensor(0.5), torch.tensor(1.0)))
+    with torch.no_grad():
+        assert torch.equal(fused_post_norm(t["x"], t["r"], residual_scale=p), fused_post_norm(t["x"], t["r"], residual_scale=0.5))
