@@ -383,9 +383,11 @@ quant_ring_kernel(const __grid_constant__ NormParams p, int stages) {
   }
 }
 
-// Backward.  With e = dh + rstd(h) w' dn and c = rstd(h)^3 mean(w' dn h) the gradient that reaches h is e - c h, and the
-// sum that the norm of y needs, sum(w y g (e - c h)), is A - c B with A = sum(w y g e), B = sum(w y g h): all three sums
+// Backward.  With k = h rstd(h), e = dh + rstd(h) w' dn and c = rstd(h) mean(w' dn k) the gradient that reaches h is e - c k, and
+// the sum that the norm of y needs, S = sum(w y g (e - c k)), is A - c B with A = sum(w y g e), B = sum(w y g k): all three sums
 // of a row are formed in one reduction.  A gate per token is a factor of A and B, and its own gradient is rstd(y)(A - cB).
+// The part of dy along y is (y rstd(y)) (rstd(y) (rstd(y) S) / H).  No power of rstd is formed: its cube leaves the
+// 32-bit range where a row's RMS passes 5e12, while the row's sum of squares stays in it up to an RMS of 1.8e19 / sqrt(H).
 // The gradients of the weights and of a gate per channel are summed over the CTA's rows in registers, stored once per
 // CTA and joined by column_sum_kernel in a fixed order: no atomics, the same bits on every run.
 template <typename T, int VEC, int NV>
@@ -417,6 +419,7 @@ block_norm_bwd_kernel(const __grid_constant__ NormBwdParams b) {
       if (p.w != nullptr) ry = p.rstd[t];
       if (p.wn != nullptr) rh = p.rstd[p.T + t];
     }
+    const float yg = ry * gt, alpha_h = p.alpha * rh;
     float y[NV][VEC], h[NV][VEC], e[NV][VEC], dn[NV][VEC];
     float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
@@ -438,23 +441,22 @@ block_norm_bwd_kernel(const __grid_constant__ NormBwdParams b) {
         if (p.wn != nullptr) load_param<T, VEC>(p.wn, p.wn_f32, c, wn);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float wy = y[i][j] * w[j];
-          h[i][j] = fmaf(p.alpha, h[i][j], g[j] * (wy * ry));
+          const float v = by_value ? y[i][j] * w[j] * g[j] : y[i][j] * w[j];
+          h[i][j] = fmaf(alpha_h, h[i][j], v * yg * rh);          // h rstd(h)
           const float wd = wn[j] * dn[i][j];
           e[i][j] = fmaf(rh, wd, e[i][j]);
           s[0] = fmaf(wd, h[i][j], s[0]);
-          const float v = by_value ? wy * g[j] : wy;
           s[1] = fmaf(v, e[i][j], s[1]);
           s[2] = fmaf(v, h[i][j], s[2]);
         }
       }
     }
     red.sum(s);
-    const float c3 = rh * rh * rh * s[0] * inv_h;
-    const float raw = s[1] - c3 * s[2];
-    const float cy = (p.w != nullptr) ? ry * ry * ry * (by_value ? raw : gt * raw) * inv_h : 0.f;
+    const float c1 = rh * s[0] * inv_h;
+    const float sum_y = ry * (s[1] - c1 * s[2]);
+    const float cy = (p.w != nullptr) ? yg * sum_y * inv_h : 0.f;
     if (row && threadIdx.x == 0 && p.gate_kind == B200MOE_GATE_TOKEN && b.dgate != nullptr) {
-      const float one[1] = {ry * raw};
+      const float one[1] = {sum_y};
       store_param<T, 1>(b.dgate, p.gate_f32, t, one);
     }
 #pragma unroll
@@ -468,12 +470,12 @@ block_norm_bwd_kernel(const __grid_constant__ NormBwdParams b) {
         if (p.w != nullptr) load_param<T, VEC>(p.w, p.w_f32, c, w);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float d = fmaf(-c3, h[i][j], e[i][j]);
+          const float d = fmaf(-c1, h[i][j], e[i][j]);
           dr[j] = p.alpha * d;
           const float du = d * g[j], yr = y[i][j] * ry;
-          out[j] = fmaf(ry * w[j], du, -cy * y[i][j]);
+          out[j] = fmaf(ry * w[j], du, -cy * yr);
           aw[i][j] = fmaf(du, yr, aw[i][j]);
-          an[i][j] = fmaf(dn[i][j], h[i][j] * rh, an[i][j]);
+          an[i][j] = fmaf(dn[i][j], h[i][j], an[i][j]);
           const float dg = d * (yr * w[j]);
           ag[i][j] += dg;
           g[j] = dg;
@@ -639,11 +641,11 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
       }
     float t0 = both_of(s0), t1 = both_of(s1), t2 = both_of(s2);
     if (POST || NEXT || token) red.sum3(t0, t1, t2);
-    const float c1 = NEXT ? rh * t0 * inv_h : 0.f;          // rstd(h)^3 mean(w' dn h) h = c1 (h rstd(h))
-    const float raw = t1 - c1 * t2;
-    const float cy = POST ? ry * ry * ry * gt * raw * inv_h : 0.f;
+    const float c1 = NEXT ? rh * t0 * inv_h : 0.f;
+    const float sum_y = ry * (t1 - c1 * t2);
+    const float cy = POST ? ry * sum_y * inv_h : 0.f;       // of y rstd(y) gate
     if (token && tid == 0 && b.dgate != nullptr) {
-      const float one[1] = {ry * raw};
+      const float one[1] = {sum_y};
       store_param<T, 1>(b.dgate, p.gate_f32, t, one);
     }
     const f32x2 c2 = both(-c1), cy2 = both(-cy), alpha2 = both(p.alpha), yg2 = both(ry * gt);
@@ -679,8 +681,9 @@ block_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams b) {
         if (POST) {
 #pragma unroll
           for (int j = 0; j < N2; ++j) {
-            aw[i][j] = fma2(d[j], mul2(y[j], yg2), aw[i][j]);
-            d[j] = fma2(d[j], mul2(f[j], yg2), mul2(y[j], cy2));
+            const f32x2 yr = mul2(y[j], yg2);
+            aw[i][j] = fma2(d[j], yr, aw[i][j]);
+            d[j] = fma2(d[j], mul2(f[j], yg2), mul2(yr, cy2));
           }
         } else if (GATE == 0) {
 #pragma unroll

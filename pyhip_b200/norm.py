@@ -49,7 +49,7 @@ def fused_post_norm(y, residual, weight=None, *, gate=None, residual_scale=1.0, 
 
     Arithmetic in 32 bits, each result rounded once; n is the norm of the unrounded h.  Differentiable in all five tensors, in
     reverse mode and once; forward-mode derivatives and tracing are refused.  Gradients that sum over tokens are added in a fixed
-    order.
+    order.  A row's sum of squares is a 32-bit number too: an RMS of more than 1.8e19 / sqrt(H) makes its rstd 0, as in torch.
     Returns h; (h, n) with ``next_weight``; (h, q, scale) with ``quant`` as well."""
     if residual is None:
         raise ValueError("fused_post_norm needs the residual")
