@@ -20,6 +20,7 @@
 extern "C" {
 #endif
 
+/* changes with the arguments of an entry or the layout of a struct; entries are added without */
 #define B200MOE_VERSION 3
 
 /* weight formats */

@@ -118,9 +118,14 @@ def lib() -> ctypes.CDLL:
         raise ImportError(f"{LIB_PATH} is missing: run `python -c 'import __graft_entry__ as g; g.build()'` "
                           "(needs nvcc); this package has no CPU or eager fallback")
     L = ctypes.CDLL(str(LIB_PATH))
+    # before anything else is bound: a library of another version need not have the entries, nor these arguments
+    L.b200moe_version.restype = ctypes.c_int
+    missing = [n for n in EXPORTS if not hasattr(L, n)]
+    if missing or L.b200moe_version() != ABI_VERSION:
+        raise RuntimeError(f"libb200moe.so version mismatch; rebuild it (version {L.b200moe_version()} of {ABI_VERSION}, "
+                           f"missing: {', '.join(missing) or 'nothing'})")
     vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
     sp, wp = ctypes.POINTER(Shape), ctypes.POINTER(Workspace)
-    L.b200moe_version.restype = ctypes.c_int
     L.b200moe_last_error.restype = ctypes.c_char_p
     L.b200moe_workspace_layout.argtypes = [sp, wp]
     L.b200moe_prepared_scale_bytes.argtypes = [sp, ctypes.c_int, ctypes.POINTER(i64)]
@@ -160,8 +165,6 @@ def lib() -> ctypes.CDLL:
     for name in EXPORTS:
         if name not in ("b200moe_version", "b200moe_last_error"):
             getattr(L, name).restype = ctypes.c_int
-    if L.b200moe_version() != ABI_VERSION:
-        raise RuntimeError("libb200moe.so version mismatch; rebuild it")
     return L
 
 
