@@ -77,6 +77,18 @@ def _stale(target, deps) -> bool:
     return not target.exists() or any(target.stat().st_mtime < d.stat().st_mtime for d in deps)
 
 
+def _dense_tag() -> str:
+    """What the torch binding is built against; it stands in the file as text."""
+    import sys
+
+    import torch
+    return f"dense binding for torch {torch.__version__}, {sys.implementation.cache_tag}"
+
+
+def _dense_fits() -> bool:
+    return DENSE_PATH.exists() and f"{_dense_tag()}\0".encode() in DENSE_PATH.read_bytes()
+
+
 def _dense_command():
     import sysconfig
 
@@ -85,7 +97,7 @@ def _dense_command():
     cuda = pathlib.Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve().parents[1]
     inc = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], cuda / "include"]
     return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_dense",
-            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-DTORCH_API_INCLUDE_EXTENSION_H", f'-DB200MOE_DENSE_TAG="{_dense_tag()}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
             *(f"-isystem{i}" for i in inc), "-o", str(DENSE_PATH), str(CSRC / "dense_torch.cpp"), f"-L{root / 'lib'}", "-lc10",
             "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", f"-L{PKG_DIR}", "-l:libb200moe.so", "-Wl,-rpath,$ORIGIN",
             f"-Wl,-rpath,{root / 'lib'}"]
@@ -105,7 +117,7 @@ def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
             raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
         if verbose:
             print(res.stderr)
-    if force or _stale(DENSE_PATH, [CSRC / "dense_torch.cpp", header]):
+    if force or _stale(DENSE_PATH, [CSRC / "dense_torch.cpp", header]) or not _dense_fits():
         res = subprocess.run(_dense_command(), capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError("g++ failed:\n" + res.stdout + res.stderr)
@@ -178,6 +190,8 @@ def dense():
     lib()                                   # the library that it links against, of the version that it was built for
     if not DENSE_PATH.exists():
         raise ImportError(f"{DENSE_PATH} is missing: run `python -c 'import __graft_entry__ as g; g.build()'`")
+    if not _dense_fits():                   # loading it could end the process
+        raise ImportError(f"{DENSE_PATH} was built for another torch or Python than this one ({_dense_tag()}): rebuild it")
     import importlib.util
 
     import torch  # noqa: F401  (its libraries have to be loaded first)

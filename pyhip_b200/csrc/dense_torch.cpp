@@ -21,6 +21,9 @@
 
 #include "../../include/b200moe.h"
 
+// the torch and the Python that this file was built for, to be read without loading it
+extern "C" __attribute__((visibility("default"), used)) const char b200moe_dense_tag[] = B200MOE_DENSE_TAG;
+
 namespace {
 
 using at::Tensor;

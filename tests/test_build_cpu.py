@@ -19,3 +19,18 @@ def test_a_library_of_another_version_says_so(tmp_path, monkeypatch, names, vers
     monkeypatch.setattr(_lib, "LIB_PATH", _stub(tmp_path, names, version))
     with pytest.raises(RuntimeError, match="rebuild"):
         _lib.lib.__wrapped__()
+
+
+def test_a_binding_for_another_torch_is_rebuilt_and_not_loaded(monkeypatch):
+    import torch
+    _lib.build()
+    assert _lib._dense_fits() and _lib.dense.__wrapped__() is not None
+    ran = []
+    monkeypatch.setattr(_lib.subprocess, "run", lambda cmd, **_: ran.append(cmd) or subprocess.CompletedProcess(cmd, 0, "", ""))
+    _lib.build()
+    assert not ran
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    _lib.build()
+    assert len(ran) == 1 and str(_lib.DENSE_PATH) in ran[0]
+    with pytest.raises(ImportError, match="rebuild"):
+        _lib.dense.__wrapped__()
