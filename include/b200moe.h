@@ -328,12 +328,18 @@ int b200moe_quantize_int8(const void* x, int64_t x_stride, int32_t T, int32_t K,
  *   x          i8 [T, K] (x_dtype INT8, x_stride = K, with x_scale [T]) or bf16 / fp16 / fp32 rows, which are quantised
  *              first into workspace (b200moe_linear_int8_workspace bytes, 16-byte aligned; unused for INT8)
  *   weight     i8 [N, K], 16-byte aligned;  weight_scale f32 [N];  bias f32 [N] or NULL
- *   variant    0 = by size, 1 = split-K tiles for few tokens, 2 = CTA pairs
- *   status     i32 [2] or NULL: word 0 = id of a bounded wait that ran out (left alone otherwise), word 1 = CTA */
+ *   variant    0 = by size, 1 = split-K tiles for few tokens, 2 = CTA pairs; plus B200MOE_LINEAR_HOLD_BACK to leave out one
+ *              weight copy, so that the waits behind it run out after two seconds (for tests of what they leave)
+ *   status     i32 [2]: word 0 = id of a bounded wait that ran out (left alone otherwise), word 1 = CTA; NULL for the
+ *              library's own words of the device */
+#define B200MOE_LINEAR_HOLD_BACK 256
 int b200moe_linear_int8_workspace(int32_t T, int32_t N, int32_t K, int32_t variant, int64_t* bytes);
 int b200moe_linear_int8(const void* x, int64_t x_stride, int32_t x_dtype, const float* x_scale, const void* weight,
                         const float* weight_scale, const float* bias, int32_t T, int32_t N, int32_t K, int32_t out_dtype,
                         int32_t variant, void* workspace, int64_t workspace_bytes, int32_t* status, void* y, void* stream);
+/* The library's words of the current device, which calls without words of their own leave (0, 0 if no wait ever ran out).
+ * Synchronises the device. */
+int b200moe_linear_int8_status(int32_t* status_host2);
 
 /* RMS norms after and before a block, fused with the branch's gate and the residual:
  *   u = y * rstd(y) * weight (u = y without weight);  h = residual_scale * residual + gate * u;  n = h * rstd(h) * next_weight

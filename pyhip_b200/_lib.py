@@ -33,6 +33,7 @@ COMBINE_GATHER, COMBINE_FUSED = 0, 1
 ACTQ_TERMS, ACTQ_1X128 = 0, 1
 ABI_VERSION = 3
 T_BF16, T_FP16, T_FP32, T_INT8 = 0, 1, 2, 3
+LINEAR_HOLD_BACK = 256
 GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = 0, 1, 2, 3
 
 
@@ -68,7 +69,7 @@ EXPORTS = ["b200moe_version", "b200moe_last_error", "b200moe_workspace_layout",
            "b200moe_sort_scratch_bytes", "b200moe_route_topk", "b200moe_forward_static", "b200moe_gather_sum", "b200moe_debug_probe",
            "b200moe_forward_ex", "b200moe_static_status", "b200moe_ep_plan", "b200moe_quant_rows_fp8_1x128",
            "b200moe_forward_batch1", "b200moe_batch1_scratch_bytes",
-           "b200moe_quantize_int8", "b200moe_linear_int8", "b200moe_linear_int8_workspace", "b200moe_block_norm", "b200moe_block_norm_bwd",
+           "b200moe_quantize_int8", "b200moe_linear_int8", "b200moe_linear_int8_workspace", "b200moe_linear_int8_status", "b200moe_block_norm", "b200moe_block_norm_bwd",
            "b200moe_block_norm_bwd_workspace", "b200moe_router_workspace", "b200moe_router_forward",
            "b200moe_router_backward"]
 
@@ -168,6 +169,7 @@ def lib() -> ctypes.CDLL:
     L.b200moe_quantize_int8.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp]
     L.b200moe_linear_int8.argtypes = [vp, i64, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, vp, vp, vp]
     L.b200moe_linear_int8_workspace.argtypes = [i32, i32, i32, i32, ctypes.POINTER(i64)]
+    L.b200moe_linear_int8_status.argtypes = [ctypes.POINTER(i32)]
     L.b200moe_block_norm.argtypes = norm + [f32] + [vp] * 6
     L.b200moe_block_norm_bwd.argtypes = norm + [vp] * 8 + [vp, i64, vp]
     L.b200moe_block_norm_bwd_workspace.argtypes = [i32, i32, i32, ctypes.POINTER(i64)]

@@ -9,12 +9,10 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-#include <cuda_runtime_api.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <initializer_list>
-#include <mutex>
 #include <optional>
 #include <string>
 #include <vector>
@@ -144,32 +142,6 @@ std::tuple<Tensor, Tensor> quantize_int8(const Tensor& x) {
   return {q, scale};
 }
 
-// Status words of linear_int8, one pair per device, kept until the process ends.  None while a graph is being captured and
-// they do not exist yet: a graph's memory would not outlive it.
-std::mutex status_lock;
-std::vector<Tensor>& status_words() {
-  static auto* v = new std::vector<Tensor>(64);
-  return *v;
-}
-int32_t* status_of(const Tensor& x, void* stream) {
-  std::lock_guard<std::mutex> hold(status_lock);
-  auto& all = status_words();
-  const size_t i = (size_t)x.get_device();
-  if (i >= all.size()) return nullptr;
-  if (!all[i].defined()) {
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing((cudaStream_t)stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) return nullptr;
-    all[i] = at::zeros({2}, x.options().dtype(at::kInt).requires_grad(false));
-  }
-  return all[i].data_ptr<int32_t>();
-}
-OptTensor int8_status(int64_t device) {
-  std::lock_guard<std::mutex> hold(status_lock);
-  auto& all = status_words();
-  if (device < 0 || (size_t)device >= all.size() || !all[(size_t)device].defined()) return std::nullopt;
-  return all[(size_t)device];
-}
-
 Tensor linear_int8(const Tensor& x, const Tensor& weight, const Tensor& weight_scale, const OptTensor& x_scale, const OptTensor& bias,
                    std::optional<at::ScalarType> out_dtype, int64_t variant) {
   need_cuda(x, "linear_int8");
@@ -220,7 +192,7 @@ Tensor linear_int8(const Tensor& x, const Tensor& weight, const Tensor& weight_s
   if ((uintptr_t)ptr(w) & 15) w = w.clone();
   const Tensor sc = packed(weight_scale), b = bias ? packed(*bias) : Tensor();
   call_check(b200moe_linear_int8(ptr(r.t), r.stride, dt, (const float*)ptr(xs), ptr(w), (const float*)ptr(sc), (const float*)ptr(b), T, n,
-                                 (int32_t)K, row_type(out), (int32_t)variant, ptr(ws), bytes, status_of(x, stream), ptr(y), stream),
+                                 (int32_t)K, row_type(out), (int32_t)variant, ptr(ws), bytes, nullptr, ptr(y), stream),
              "linear_int8");
   return y;
 }
@@ -481,7 +453,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   using no_gil = py::call_guard<py::gil_scoped_release>;
   m.def("quantize_int8", &quantize_int8, no_gil());
   m.def("linear_int8", &linear_int8, no_gil());
-  m.def("int8_status", &int8_status);
   m.def("block_norm", &block_norm, no_gil());
   m.def("router", &router, no_gil());
 }

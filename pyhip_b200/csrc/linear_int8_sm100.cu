@@ -54,9 +54,19 @@ struct LinearParams {
   int32_t* status;
   const void* x;        // the row that the split kernel quantises itself
   int T, N, K, KB, k_tail_steps, stages, fp16, store_tma, early_weights, x_dtype, x_vec;
+  int hold_back;                  // the CTAs (along x) that leave out their last weight copy (-1: none), for tests of the waits
   int tokens, splits;             // split: token tile, CTAs that share K
   int m_tiles, n_tiles;           // pair
 };
+
+// Where a bounded wait that ran out is reported if the caller gives no words of its own: one pair per device, zero when the library
+// is loaded, there for calls that are captured too, and never cleared.
+__device__ int32_t g_linear_status[2];
+__device__ __forceinline__ void report_abort(const LinearParams& p, uint32_t word) {
+  int32_t* s = p.status != nullptr ? p.status : g_linear_status;
+  s[0] = (int32_t)word;
+  s[1] = (int32_t)blockIdx.x;
+}
 
 struct SmemCtlI8 {
   uint64_t full[kMaxStagesI8];
@@ -258,11 +268,12 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
       // The weights do not depend on the launch in front when that is this call's own quantiser (early_weights): it
       // lets this grid start only after everything before it has completed.
       int ahead = 0;
+      const int held = p.hold_back == (int)blockIdx.x ? kb1 - 1 : kb1;             // the k-block that is not fetched
       if (!FUSED && p.early_weights)
         for (; ahead < min(S, kb1 - kb0); ++ahead) {
           const uint32_t full = smem_u32(&ctl->full[ahead]);
           mbar_expect_tx(full, stage_bytes);
-          tma_load_2d(stage0 + ahead * stage_bytes, &p.tmW, full, (kb0 + ahead) * kTileKI8, n0);
+          if (kb0 + ahead < held) tma_load_2d(stage0 + ahead * stage_bytes, &p.tmW, full, (kb0 + ahead) * kTileKI8, n0);
         }
       grid_dep_wait();
       int64_t issued = 0;
@@ -273,7 +284,7 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
         const uint32_t st = stage0 + stage * stage_bytes, full = smem_u32(&ctl->full[stage]);
         if (kb - kb0 >= ahead) {
           mbar_expect_tx(full, stage_bytes);
-          tma_load_2d(st, &p.tmW, full, kb * kTileKI8, n0);
+          if (kb < held) tma_load_2d(st, &p.tmW, full, kb * kTileKI8, n0);
         }
         if (!FUSED) tma_load_2d(st + kRowTileBytes, &p.tmX, full, kb * kTileKI8, t0);
         ++issued;
@@ -384,10 +395,7 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
       }
     }
   }
-  if (threadIdx.x == 0 && ctl->abort_word != 0 && p.status != nullptr) {
-    p.status[0] = (int32_t)ctl->abort_word;
-    p.status[1] = (int32_t)blockIdx.x;
-  }
+  if (threadIdx.x == 0 && ctl->abort_word != 0) report_abort(p, ctl->abort_word);
   __syncwarp();
   cluster_sync_all();                // no CTA leaves while another one reads its tile
   if (warp == 1) tmem_dealloc(tmem_base, cols);
@@ -465,6 +473,7 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
       uint32_t phase = 0;
       int64_t issued = 0;
       bool ok = true;
+      const int held = p.hold_back == (int)blockIdx.x ? kb1 - 1 : kb1;
       for (int w = first; w < total && ok; w += step) {
         int m, n;
         tile_of(w, p.m_tiles, p.n_tiles, m, n);
@@ -474,7 +483,7 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
           const uint32_t st = stage0 + stage * STAGE, full = smem_u32(&ctl->full[stage]);
           if (rank == 0) mbar_expect_tx(full, 2 * STAGE);
           tma_load_2d_pair(st, &p.tmX, full, kb * kTileKI8, t0);
-          tma_load_2d_pair(st + kRowTileBytes, &p.tmW, full, kb * kTileKI8, n0);
+          if (kb < held) tma_load_2d_pair(st + kRowTileBytes, &p.tmW, full, kb * kTileKI8, n0);
           ++issued;
           if (++stage == S) { stage = 0; phase ^= 1; }
         }
@@ -634,10 +643,7 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (threadIdx.x == 0 && ctl->abort_word != 0 && p.status != nullptr) {
-    p.status[0] = (int32_t)ctl->abort_word;
-    p.status[1] = (int32_t)blockIdx.x;
-  }
+  if (threadIdx.x == 0 && ctl->abort_word != 0) report_abort(p, ctl->abort_word);
   cluster_sync_all();     // neither CTA leaves while the other's products or arrivals may still touch it
   if (warp == 1) tmem_dealloc_pair(tmem_base, COLS);
 }
@@ -699,6 +705,7 @@ struct LinearArgs {
   void* y;
   int T, N, K, fp16, early_weights;
   int32_t* status;
+  bool hold_back;
 };
 int launch_linear_int8(const LinearArgs& a, const Variant& v, cudaStream_t st) {
   LinearParams p;
@@ -708,6 +715,7 @@ int launch_linear_int8(const LinearArgs& a, const Variant& v, cudaStream_t st) {
   p.KB = (K + kTileKI8 - 1) / kTileKI8;
   p.k_tail_steps = (K - (p.KB - 1) * kTileKI8 + 31) / 32;
   p.T = T; p.N = N; p.x_scale = a.x_scale; p.w_scale = a.w_scale; p.bias = a.bias; p.y = a.y; p.status = a.status; p.fp16 = a.fp16;
+  p.hold_back = a.hold_back ? (v.pair ? 1 : 0) : -1;      // of a pair, the CTA that does not issue the products
   if (!v.pair) {
     p.tokens = v.tokens; p.splits = v.splits; p.stages = v.stages; p.early_weights = a.early_weights;
     p.x = a.x; p.x_dtype = a.x_dtype;
@@ -761,7 +769,15 @@ int launch_linear_int8(const LinearArgs& a, const Variant& v, cudaStream_t st) {
 
 using namespace b200moe;
 
+extern "C" int b200moe_linear_int8_status(int32_t* status2) {
+  B200_CHECK_ARG(status2 != nullptr, "linear_int8_status: NULL pointer");
+  B200_CHECK_CUDA(cudaDeviceSynchronize());
+  B200_CHECK_CUDA(cudaMemcpyFromSymbol(status2, g_linear_status, 2 * sizeof(int32_t)));
+  return 0;
+}
+
 extern "C" int b200moe_linear_int8_workspace(int32_t T, int32_t N, int32_t K, int32_t variant, int64_t* bytes) {
+  variant &= ~B200MOE_LINEAR_HOLD_BACK;
   B200_CHECK_ARG(bytes != nullptr && T >= 0 && N >= 1 && K >= 1 && variant >= 0 && variant <= 2, "linear_int8_workspace: T=%d N=%d K=%d", T, N, K);
   const Variant v = pick_variant(T, N, K, variant, true);
   *bytes = T == 0 || v.fused ? 0 : round_up64((int64_t)T * K, 256) + (int64_t)T * 4;     // the quantised rows and their scales
@@ -775,6 +791,8 @@ extern "C" int b200moe_linear_int8(const void* x, int64_t x_stride, int32_t x_dt
                  T, N, K);
   B200_CHECK_ARG(out_dtype == B200MOE_T_BF16 || out_dtype == B200MOE_T_FP16, "linear_int8: out dtype %d", out_dtype);
   B200_CHECK_ARG(x_dtype == B200MOE_T_INT8 || (x_dtype >= B200MOE_T_BF16 && x_dtype <= B200MOE_T_FP32), "linear_int8: x dtype %d", x_dtype);
+  const bool hold_back = (variant & B200MOE_LINEAR_HOLD_BACK) != 0;
+  variant &= ~B200MOE_LINEAR_HOLD_BACK;
   B200_CHECK_ARG(variant >= 0 && variant <= 2, "linear_int8: variant %d", variant);
   if (T == 0) return 0;
   B200_CHECK_ARG(x && weight && weight_scale && y, "linear_int8: NULL pointer");
@@ -783,7 +801,7 @@ extern "C" int b200moe_linear_int8(const void* x, int64_t x_stride, int32_t x_dt
   cudaStream_t st = (cudaStream_t)stream;
   const bool quantise = x_dtype != B200MOE_T_INT8;
   const Variant v = pick_variant(T, N, K, variant, quantise);
-  LinearArgs a = {x, x_dtype, x, x_scale, weight, weight_scale, bias, y, T, N, K, out_dtype == B200MOE_T_FP16, quantise, status};
+  LinearArgs a = {x, x_dtype, x, x_scale, weight, weight_scale, bias, y, T, N, K, out_dtype == B200MOE_T_FP16, quantise, status, hold_back};
   if (!quantise) {
     B200_CHECK_ARG(x_scale != nullptr && x_stride == K && ((uintptr_t)x & 15) == 0, "linear_int8: 8-bit rows must be contiguous, 16-byte aligned and have x_scale");
   } else {

@@ -118,11 +118,15 @@ def quantize_int8(x):
 
 
 def int8_status(device=None):
-    """Host read of the error words that `linear_int8` calls on ``device`` leave (synchronises; for tests and debugging):
-    (id of the barrier wait that ran out, its CTA), (0, 0) if none ever did."""
-    index = None if device is None else torch.device(device).index
-    t = _lib.dense().int8_status(torch.cuda.current_device() if index is None else index)
-    return (0, 0) if t is None else tuple(t.cpu().tolist())
+    """Host read of the error words that `linear_int8` calls on ``device`` leave, captured ones too (synchronises; for tests and
+    debugging): (id of the barrier wait that ran out, its CTA), (0, 0) if none ever did."""
+    d = torch.device("cuda" if device is None else device if not isinstance(device, int) else f"cuda:{device}")
+    if d.type != "cuda":
+        raise ValueError(f"device={device!r}: a CUDA device")
+    words = (ctypes.c_int32 * 2)()
+    with torch.cuda.device(d):
+        _lib.check(_lib.lib().b200moe_linear_int8_status(words), "linear_int8_status")
+    return tuple(words)
 
 
 def linear_int8(x, weight, weight_scale, *, x_scale=None, bias=None, out_dtype=None, variant: int = 0):
