@@ -331,7 +331,7 @@ int b200moe_quantize_int8(const void* x, int64_t x_stride, int32_t T, int32_t K,
  *   variant    0 = by size, 1 = split-K tiles for few tokens, 2 = CTA pairs; plus B200MOE_LINEAR_HOLD_BACK to leave out one
  *              weight copy, so that the waits behind it run out after two seconds (for tests of what they leave)
  *   status     i32 [2]: word 0 = id of a bounded wait that ran out (left alone otherwise), word 1 = CTA; NULL for the
- *              library's own words of the device */
+ *              library's own words of the device.  What depends on the missing data is NaN in y */
 #define B200MOE_LINEAR_HOLD_BACK 256
 int b200moe_linear_int8_workspace(int32_t T, int32_t N, int32_t K, int32_t variant, int64_t* bytes);
 int b200moe_linear_int8(const void* x, int64_t x_stride, int32_t x_dtype, const float* x_scale, const void* weight,

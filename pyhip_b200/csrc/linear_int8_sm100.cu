@@ -18,8 +18,8 @@
 // ones: start and first load 2, the last tile's way out and the join 3 to 4.
 //
 // A pipeline stage is 128 bytes of K (one swizzle span): 128 rows of one operand and BT or BN/2 rows of the other, one TMA
-// copy each; K and row tails are zero-filled by the copy.  Every barrier wait is bounded; one that runs out sets status[]
-// and the CTA unwinds and frees its tensor memory.
+// copy each; K and row tails are zero-filled by the copy.  Every barrier wait is bounded; one that runs out sets status[],
+// what its sums belong to becomes NaN, and the CTA unwinds and frees its tensor memory.
 #include <string.h>
 
 #include <algorithm>
@@ -75,6 +75,7 @@ struct SmemCtlI8 {
   uint64_t tmem_empty[2];
   uint32_t tmem_base;
   uint32_t abort_word;
+  uint32_t peer_lost;             // a CTA of the cluster has no sums to give
 };
 static_assert(sizeof(SmemCtlI8) <= kCtlBytes, "control block");
 
@@ -135,6 +136,14 @@ __device__ __forceinline__ int4 ld_peer_v4(uint32_t addr) {
   int4 v;
   asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
+}
+__device__ __forceinline__ uint32_t ld_peer_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_peer_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void st_peer_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -343,7 +352,7 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
   for (int j = 0; j < 4; ++j) xs_of[j] = (!FUSED && j * 32 + lane < live) ? p.x_scale[t0 + j * 32 + lane] : 0.f;
   // the tile as [token][feature] int32 in the stages' memory, which the products no longer need
   if (warp >= 2) {
-    ok = mbar_wait(smem_u32(&ctl->tmem_full[0]), 0, abort_word, 0x1300);
+    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->tmem_full[0]), 0, abort_word, 0x1300));
     if (ok) {
       tc_fence_after_sync();
       const int quad = warp & 3;
@@ -363,6 +372,8 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
   tc_fence_after_sync();
   // token columns are dealt out over the cluster's warps; a lane adds four neighbouring features of all its CTAs.  Four
   // columns at a time: a load from another CTA takes hundreds of cycles.
+  // A CTA whose wait ran out has no sums to give: the cluster's tile becomes NaN, as a row that cannot be quantised does.
+  const bool lost = __any_sync(0xffffffffu, lane < C && ld_peer_u32(peer_smem(smem_u32(&ctl->abort_word), (uint32_t)min(lane, C - 1))) != 0);
   const int stride = C * (kThreadsI8 / 32);
   for (int c0 = rank + C * warp; c0 < live; c0 += 4 * stride) {
     int4 a[4];
@@ -380,7 +391,8 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
     for (int q = 0; q < 4; ++q) {
       const int c = c0 + q * stride;
       if (c >= live) break;                                  // (the same for the whole warp)
-      const float xs = FUSED ? row_scale : __shfl_sync(0xffffffffu, c < 32 ? xs_of[0] : c < 64 ? xs_of[1] : c < 96 ? xs_of[2] : xs_of[3], c & 31);
+      float xs = FUSED ? row_scale : __shfl_sync(0xffffffffu, c < 32 ? xs_of[0] : c < 64 ? xs_of[1] : c < 96 ? xs_of[2] : xs_of[3], c & 31);
+      if (lost) xs = __uint_as_float(0x7fc00000u);
       const float o0 = fmaf((float)a[q].x * xs, ws[0], bs[0]), o1 = fmaf((float)a[q].y * xs, ws[1], bs[1]);
       const float o2 = fmaf((float)a[q].z * xs, ws[2], bs[2]), o3 = fmaf((float)a[q].w * xs, ws[3], bs[3]);
       const uint32_t lo = pack2(o0, o1, p.fp16), hi = pack2(o2, o3, p.fp16);
@@ -448,6 +460,7 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
       mbar_init(smem_u32(&ctl->tmem_empty[a]), 16);         // the epilogue warps of both CTAs
     }
     ctl->abort_word = 0;
+    ctl->peer_lost = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
   }
@@ -537,7 +550,7 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
       int m, n;
       tile_of(first, p.m_tiles, p.n_tiles, m, n);
       load_scales(n * BN, 0);
-      ready = mbar_wait(smem_u32(&ctl->tmem_full[0]), 0, abort_word, 0x2400);
+      ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->tmem_full[0]), 0, abort_word, 0x2400));
     }
     __syncwarp();
     tc_fence_before_sync();
@@ -557,14 +570,17 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
         }
       }
     }
+    if (warp >= 2 && !ready && lane < 2 * Z) st_peer_u32(peer_smem(smem_u32(&ctl->peer_lost), (uint32_t)lane), 1);
     __syncwarp();
     cluster_sync_all();
+    ready = ready && *(volatile uint32_t*)&ctl->peer_lost == 0;
   }
   if (warp >= 2) {
     const uint32_t mine = staging + (uint32_t)(warp - 2) * kStagingBytes;
-    int acc = 0;
+    int acc = 0, w = first;
     uint32_t acc_phase = 0;
-    for (int w = first; w < total; w += step) {
+    const int first_col = Z > 1 ? (int)z * (BN / Z) : 0;
+    for (; w < total; w += step) {
       int m, n;
       tile_of(w, p.m_tiles, p.n_tiles, m, n);
       const int row0 = m * 256 + (int)rank * 128 + quad * 32, n0 = n * BN;
@@ -578,7 +594,6 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
       if (!all) break;
       tc_fence_after_sync();
       const uint32_t tacc = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN;
-      const int first_col = Z > 1 ? (int)z * (BN / Z) : 0;
 #pragma unroll 1
       for (int c0 = first_col + half * kStoreCols; c0 < first_col + BN / Z; c0 += 2 * kStoreCols) {
         if (row0 >= p.T || n0 + c0 >= p.N) break;
@@ -637,6 +652,15 @@ linear_int8_pair_kernel(const __grid_constant__ LinearParams p) {
       if (acc == 0) acc_phase ^= 1;
     }
     if (lane == 0) bulk_wait_all();
+    // A wait ran out: the tiles that are left become NaN, as a row that cannot be quantised does.
+    for (; w < total; w += step) {
+      int m, n;
+      tile_of(w, p.m_tiles, p.n_tiles, m, n);
+      const int row0 = m * 256 + (int)rank * 128 + quad * 32;
+      for (int r = row0; r < min(row0 + 32, p.T); ++r)
+        for (int c = n * BN + first_col + half * 32 + lane; c < min(n * BN + first_col + BN / Z, p.N); c += 64)
+          static_cast<uint16_t*>(p.y)[(int64_t)r * p.N + c] = p.fp16 ? 0x7e00 : 0x7fc0;
+    }
   }
 
   __syncwarp();

@@ -119,7 +119,8 @@ def quantize_int8(x):
 
 def int8_status(device=None):
     """Host read of the error words that `linear_int8` calls on ``device`` leave, captured ones too (synchronises; for tests and
-    debugging): (id of the barrier wait that ran out, its CTA), (0, 0) if none ever did."""
+    debugging): (id of the barrier wait that ran out, its CTA), (0, 0) if none ever did.  A call whose wait ran out returns NaN
+    in the tiles that depend on it."""
     d = torch.device("cuda" if device is None else device if not isinstance(device, int) else f"cuda:{device}")
     if d.type != "cuda":
         raise ValueError(f"device={device!r}: a CUDA device")
