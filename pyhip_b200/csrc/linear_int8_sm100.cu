@@ -36,6 +36,7 @@ constexpr int kTileKI8 = 128;                   // bytes of K per stage
 constexpr int kRowTile = 128;                   // rows of the M-side operand per CTA
 constexpr int kRowTileBytes = kRowTile * kTileKI8;
 constexpr int kMaxStagesI8 = 12;
+constexpr int kMaxTokenTile = 128;              // split: a lane holds a token column's scale for every 32 of them
 constexpr int kSmemLimitI8 = 232448;            // 227 KB
 constexpr int kCtlBytes = 1024;
 constexpr int kPairThreads = 320;               // the same with eight epilogue warps, 2-9
@@ -244,7 +245,7 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
   const int S = p.stages, BT = p.tokens, C = p.splits;
   const uint32_t stage_bytes = (uint32_t)(kRowTileBytes + (FUSED ? 0 : BT * kTileKI8));
   const uint32_t token_tiles = stage0 + S * stage_bytes;   // FUSED: one for each k-block of the CTA
-  const uint32_t cols = (uint32_t)max(32, BT);             // BT is 16 or a power of two from 32 to 256
+  const uint32_t cols = (uint32_t)max(32, BT);             // BT is 16, 32, 64 or 128
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)(blockIdx.x % (unsigned)C);        // clusters run along x
   const int n0 = (int)(blockIdx.x / (unsigned)C) * kRowTile, t0 = (int)blockIdx.y * BT;
@@ -342,14 +343,14 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
   grid_dep_wait();
   const int live = min(BT, p.T - t0);
   const int n = n0 + lane * 4;
-  float ws[4], bs[4], xs_of[4];
+  float ws[4], bs[4], xs_of[kMaxTokenTile / 32];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     ws[j] = n + j < p.N ? p.w_scale[n + j] : 0.f;
     bs[j] = (p.bias != nullptr && n + j < p.N) ? p.bias[n + j] : 0.f;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) xs_of[j] = (!FUSED && j * 32 + lane < live) ? p.x_scale[t0 + j * 32 + lane] : 0.f;
+  for (int j = 0; j < kMaxTokenTile / 32; ++j) xs_of[j] = (!FUSED && j * 32 + lane < live) ? p.x_scale[t0 + j * 32 + lane] : 0.f;
   // the tile as [token][feature] int32 in the stages' memory, which the products no longer need
   if (warp >= 2) {
     ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->tmem_full[0]), 0, abort_word, 0x1300));
@@ -709,7 +710,7 @@ Variant pick_variant(int T, int N, int K, int force, bool quantise) {
       }
     return v;
   }
-  v.tokens = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  v.tokens = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : kMaxTokenTile;
   const int64_t tiles = (int64_t)((N + kRowTile - 1) / kRowTile) * ((T + v.tokens - 1) / v.tokens);
   v.splits = 1;
   while (v.splits < 8 && tiles * v.splits * 2 <= 3 * sms && KB / (v.splits * 2) >= 2) v.splits *= 2;
@@ -741,6 +742,7 @@ int launch_linear_int8(const LinearArgs& a, const Variant& v, cudaStream_t st) {
   p.T = T; p.N = N; p.x_scale = a.x_scale; p.w_scale = a.w_scale; p.bias = a.bias; p.y = a.y; p.status = a.status; p.fp16 = a.fp16;
   p.hold_back = a.hold_back ? (v.pair ? 1 : 0) : -1;      // of a pair, the CTA that does not issue the products
   if (!v.pair) {
+    B200_CHECK_ARG(v.tokens <= kMaxTokenTile, "linear_int8: token tile %d", v.tokens);
     p.tokens = v.tokens; p.splits = v.splits; p.stages = v.stages; p.early_weights = a.early_weights;
     p.x = a.x; p.x_dtype = a.x_dtype;
     p.x_vec = ((uintptr_t)a.x & 15) == 0;
