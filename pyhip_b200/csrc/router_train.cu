@@ -489,8 +489,10 @@ struct RouterLayout {
 };
 RouterLayout router_layout(int T, int E, int S) {
   RouterLayout r;
-  // chunks small enough to spread a few thousand rows over the SMs, and few enough that the second launch has little to add
-  const int per = (T + 2 * 148 - 1) / (2 * 148);
+  // chunks small enough to spread a few thousand rows over the SMs twice, and few enough that the second launch has little to
+  // add; their number is part of the order in which a device adds
+  const int want = 2 * device_sm_count();
+  const int per = (int)(((int64_t)T + want - 1) / want);
   r.rows = std::min(std::max((per + 7) / 8 * 8, 8), 128);
   r.chunks = (T + r.rows - 1) / r.rows;
   r.slots = (int64_t)r.chunks + S;
