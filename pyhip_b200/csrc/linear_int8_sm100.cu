@@ -367,10 +367,19 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
       }
     }
   }
+  // Tensor memory goes back before the CTA waits for the others of its cluster: an allocation blocks until there are columns, so a
+  // CTA that kept its own here could wait for one that never gets any.  Warp 1 has nothing to hand over and frees them meanwhile.
   __syncwarp();
   tc_fence_before_sync();
-  cluster_sync_all();
-  tc_fence_after_sync();
+  if (warp >= 2) asm volatile("bar.arrive 2, 160;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (warp == 1) {
+    asm volatile("bar.sync 2, 160;" ::: "memory");
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, cols);
+    __syncwarp();
+  }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   // token columns are dealt out over the cluster's warps; a lane adds four neighbouring features of all its CTAs.  Four
   // columns at a time: a load from another CTA takes hundreds of cycles.
   // A CTA whose wait ran out has no sums to give: the cluster's tile becomes NaN, as a row that cannot be quantised does.
@@ -411,7 +420,6 @@ linear_int8_split_kernel(const __grid_constant__ LinearParams p) {
   if (threadIdx.x == 0 && ctl->abort_word != 0) report_abort(p, ctl->abort_word);
   __syncwarp();
   cluster_sync_all();                // no CTA leaves while another one reads its tile
-  if (warp == 1) tmem_dealloc(tmem_base, cols);
 }
 
 // ------------------------------------------------------------------------------------ pair
@@ -753,9 +761,9 @@ int launch_linear_int8(const LinearArgs& a, const Variant& v, cudaStream_t st) {
     B200_CHECK_ARG(t_tiles <= 65535, "linear_int8: %d tokens", T);
     const int stage = kRowTileBytes + (v.fused ? 0 : v.tokens * kTileKI8);
     const int blocks = v.fused ? ((p.KB + v.splits - 1) / v.splits) * kFusedBlockBytes : 0;
-    // At least the share of shared memory that its columns are of tensor memory: CTAs of this kernel that fit an SM's shared
-    // memory then fit its tensor memory too, and no cluster waits for columns that another waiting cluster holds.  And 64 KB
-    // at least, which leaves no room beside a kernel that takes all columns (those hold most of the shared memory).
+    // At least the share of shared memory that its columns are of tensor memory, and 64 KB, which leaves no room beside a CTA that
+    // takes all columns: a CTA that fits an SM finds its columns there instead of blocking in their allocation.  (It waits for no
+    // other CTA while it holds them.  The pair kernel's CTAs do; they leave 13 KB of an SM, too little for another such kernel.)
     const int share = std::max((int)((int64_t)kSmemLimitI8 * std::max(32, v.tokens) / 512), 64 * 1024);
     const int bytes = std::max({v.stages * stage + blocks, std::min(v.tokens, T) * kRowTile * 4 + 16 * kRowTile * 4, share});
     const size_t smem = 1024 + kCtlBytes + (size_t)bytes;
