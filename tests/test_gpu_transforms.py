@@ -176,3 +176,22 @@ def test_a_learned_residual_scale_is_refused():
         fused_post_norm(t["x"], t["r"], residual_scale=fw.make_dual(torch.tensor(0.5), torch.tensor(1.0)))
     with torch.no_grad():
         assert torch.equal(fused_post_norm(t["x"], t["r"], residual_scale=p), fused_post_norm(t["x"], t["r"], residual_scale=0.5))
+
+
+def test_saved_tensors_may_be_moved_or_made_again():
+    """torch's hooks on saved tensors: kept on the host, or recomputed by a checkpoint."""
+    from torch.utils.checkpoint import checkpoint
+    t = _tensors()
+    x, w, logits = (t[k].clone().requires_grad_(True) for k in ("x", "w", "logits"))
+
+    def f(x, w, logits):
+        n, h = fused_pre_norm(x, w, residual=t["r"])
+        o = fused_router(logits, 3)
+        return (fused_post_norm(n, h, w, gate=t["g"], residual_scale=0.5) * t["r"]).sum() + (o.topk_weights * t["r"][:, :3]).sum() + o.balance_loss + o.z_loss
+
+    want = torch.autograd.grad(f(x, w, logits), [x, w, logits])
+    with torch.autograd.graph.save_on_cpu():
+        loss = f(x, w, logits)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, [x, w, logits]), want))
+    loss = checkpoint(f, x, w, logits, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, [x, w, logits]), want))
