@@ -324,7 +324,7 @@ int b200moe_quantize_int8(const void* x, int64_t x_stride, int32_t T, int32_t K,
                           void* stream);
 
 /* W8A8 linear layer: y[t,n] = (sum_k q[t,k] weight[n,k]) * scale[t] * weight_scale[n] + bias[n], the sum exact in int32,
- * rounded once to out_dtype (bf16 or fp16).  K a multiple of 16 below 2^17 (up to 16384 for rows quantised here).
+ * the rest in fp32 (up to four roundings of 2^-24), then rounded to out_dtype (bf16 or fp16).  K a multiple of 16 below 2^17 (up to 16384 for rows quantised here).
  *   x          i8 [T, K] (x_dtype INT8, x_stride = K, with x_scale [T]) or bf16 / fp16 / fp32 rows, which are quantised
  *              first into workspace (b200moe_linear_int8_workspace bytes, 16-byte aligned; unused for INT8)
  *   weight     i8 [N, K], 16-byte aligned;  weight_scale f32 [N];  bias f32 [N] or NULL

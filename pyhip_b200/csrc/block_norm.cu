@@ -6,10 +6,14 @@
 //
 // Bound by memory: forward reads y and r and writes h and n (8 bytes a value in 16-bit types), backward reads
 // y, r, dh, dn and writes dy and dr (12 bytes).  The threads that share a row take the same columns of every row, in
-// 16-byte pieces, so every value is read and written once and the sums over tokens stay in registers.
+// 16-byte pieces, so every value is read and written once and the sums over tokens stay with the thread.
 // Two forms.  Plain: a row goes straight to registers; any alignment, and the better one for narrow rows.  Ring: a
 // thread copies its pieces of the next rows to shared memory while it works on the present one (it reads nothing but
 // its own copies, so no barrier), which keeps tens of KB in flight per SM where the plain form waits at every row.
+// Wide rows do not fit the plain form's registers: it spills 0.1 KB a thread forward (1025 to 4096 values off the 16-byte grid) and
+// 0.2 to 1.2 KB backward (from 4097 values on: off the grid, of two weight types, or too wide for the ring).  4096 x 4099: 406 us
+// forward, 1084 us with the backward; 4096 x 7168 of two weight types 94 and 261 us, where one type takes 44 and 125 us in the
+// ring; 2048 x 16384 52 us (ring) and 357 us.
 // On a B200 (6.55 TB/s measured): forward 8192 x 2880 33 us, 5.7 TB/s; 8192 x 4096 43 us, 6.2 TB/s; 4096 x 7168 45 us,
 // 5.3 TB/s.  Backward 4096 x 7168 80 us, 4.4 TB/s; 8192 x 4096 80-84 us, 4.8 TB/s; 16384 x 2048 83 us, 4.8 TB/s: the three
 // sums of a row end in a barrier that a CTA's warps reach together.  Quantiser 16384 x 4096 48 us, 4.1 TB/s: a row's reduction
@@ -509,6 +513,7 @@ block_norm_bwd_kernel(const __grid_constant__ NormBwdParams b) {
 // to 896 threads, since the one CTA's phases between its barriers need the warps (4096 x 7168: 79 against 88 us; a gate's
 // values and their sums do not fit there).  Weights held in registers cost more in occupancy than their loads do
 // (8192 x 4096: 90 against 80 us).
+// 896 threads leave 72 registers, which the form with both norms takes; at 1024 threads it spills with fp32 weights.
 constexpr int kWideThreads = 896;
 template <typename T, typename P, int GATE, bool POST, bool NEXT, int VALUES>
 __global__ void __launch_bounds__(VALUES == 8 ? kWideThreads : kRowThreads, 1)

@@ -139,8 +139,9 @@ int encode_map_sw(CUtensorMap* map, CUtensorMapDataType type, int rank, const vo
                   CUtensorMapL2promotion promo, const char* what);
 int device_sm_count();
 
-// Launch `kernel` so that it may begin (prologue only: every kernel of this library calls
-// grid_dep_wait() before it touches global memory) while the previous kernel in the stream drains.
+// Launch `kernel` so that it may begin while the previous kernel in the stream drains: its prologue only, since every kernel of this
+// library calls grid_dep_wait() before it touches global memory.  One exception: the split-K W8A8 kernel copies weights ahead of
+// that where the launch in front is its own call's quantiser, which lets it start only after a wait of its own.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_chained_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                                           int cluster_x, Args&&... args) {

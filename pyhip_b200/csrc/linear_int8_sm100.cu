@@ -14,7 +14,7 @@
 //
 // On a B200 (tokens, weight N x K): 1, 2880 x 2880 6.2-6.6 us; 64, 14336 x 4096 15.4 us (17.3 with the quantiser; the weights'
 // stream alone is 9); 64, 4096 x 4096 10 us; 512, 4096 x 4096 12.9 us; 1000, 2048 x 7168 17.6 us; 2048, 7168 x 4096 43 us;
-// 16384, 14336 x 4096 590 us, 3.26 POP/s, tensor pipe 89 % active.  What a call does not overlap, 6 to 7 us, bounds the small
+// 16384, 14336 x 4096 575-606 us, 3.2-3.3 POP/s (tensor pipe 89 % active at 2048 tokens, 2.95 POP/s).  What a call does not overlap, 6 to 7 us, bounds the small
 // ones: start and first load 2, the last tile's way out and the join 3 to 4.
 //
 // A pipeline stage is 128 bytes of K (one swizzle span): 128 rows of one operand and BT or BN/2 rows of the other, one TMA
@@ -700,7 +700,7 @@ Variant pick_variant(int T, int N, int K, int force, bool quantise) {
   const int KB = (K + kTileKI8 - 1) / kTileKI8;
   Variant v = {};
   const int sms = device_sm_count();
-  v.pair = force == 2 || (force == 0 && T > 64);      // T = 64: 9.8 against 10.8 us (4096 x 4096); T = 128: 12.6 against 10.9
+  v.pair = force == 2 || (force == 0 && T > 64);      // T = 64: 9.8 against 10.8 us; T = 128: 12.6 against 10.9 (4096 x 4096, the only N x K measured)
   if (v.pair) {
     // Cost of a tile shape in us, fitted to calls of one round (T = 256 to 1000, N = 2048 and 4096, K = 4096 and 7168): rounds
     // of tiles over the pairs x k-blocks x what one takes, 0.30 for 256 features and 0.216 for 128; what a call does not
