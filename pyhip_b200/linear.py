@@ -133,6 +133,7 @@ def int8_status(device=None):
 def linear_int8(x, weight, weight_scale, *, x_scale=None, bias=None, out_dtype=None, variant: int = 0):
     """W8A8 linear layer, y = (q @ weight^T) * scale[token] * weight_scale[channel] (+ bias), the integer sums exact and the
     rest in 32 bits: a sum's conversion, its two scales and the bias round by 2^-24 each, then the result once to its type.
+    (A sum times its token's scale is such a number too: rows far above 1e30 overflow there, whatever the channel's scale.)
 
       ``x``: bf16 / fp16 / fp32 [..., K], quantised per token here as `quantize_int8` does (K <= 16384), or int8 [..., K] with
         ``x_scale`` f32 [...] (from `quantize_int8` or `fused_pre_norm(..., quant="int8")`)
